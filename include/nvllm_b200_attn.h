@@ -163,7 +163,8 @@ int nvllm_b200_paged_decode_static(const void* q, const void* k_cache, const voi
  * Bit 2 (4): a prefill pipeline wait timed out.  Bit 4 (16): a sequence too long
  * for the prefill plan.  Bit 5 (32): prefill called with inconsistent
  * cu_seqlens_q / cu_seqlens_k (see nvllm_b200_varlen_prefill / _paged_prefill).
- * Bit 6 (64): an all-reduce gave up waiting for a peer's flag.
+ * Bit 6 (64): an all-reduce gave up waiting for a peer's flag.  Bit 7 (128): copy_pages
+ * left out a pair that contradicts another one.
  * This call synchronises with the device (it copies one int back).
  */
 int nvllm_b200_device_status(int* flags_host);
@@ -337,6 +338,77 @@ int nvllm_b200_allreduce_sum(const void* in, void* out, const void* residual, vo
 int nvllm_b200_allreduce_sum_emulated(void* const* in, void* const* out, void* const* residual,
                                       void* const* buffers_host, int world, int64_t count, size_t max_bytes,
                                       unsigned int epoch, int64_t max_spins, void* stream);
+
+/*
+ * ---- the 8-bit cache ----------------------------------------------------------------
+ *
+ * A cache in half the bytes: k_cache, v_cache hold e4m3 values [NB, block_size, KVH, 128] and k_scale, v_scale fp32 scales
+ * [NB, block_size / 64, KVH], one for every 64 slots and kv head; an element stands for value * scale.  It has no
+ * counterpart in the reference, whose cache is bf16 (engine/model_runner.py:176).  block_size is a multiple of 64.  The attention entry points take
+ * any finite scales; those that the store writes are powers of two.
+ *
+ * store_kvcache_q8: nvllm_b200_store_kvcache (same slot rules) into an 8-bit cache.
+ *
+ *   For every (64 slots, kv head) that the call writes to, the scale becomes 2^k with the smallest k for which the largest
+ *   finite magnitude of the rows is at most 448 * 2^k, k within -117 .. 119 -- or stays what it was where that is larger.
+ *   A call that writes the block's FIRST slot begins the block anew: the scale it had, and rows that the call does not
+ *   write, count no longer.  (A sequence fills its pages in order, so a block's first slot is written first, and again only
+ *   when the page has been given to another sequence.)  Where the scale of a block that holds rows grows, those that the
+ *   call does not write are rounded again, to e4m3(value * old scale / new scale).  A scale that is not positive counts as none.
+ *   Values are rounded to nearest even; above 448 * 2^119 they saturate.  NaN and infinities are stored as NaN.
+ *   Of several rows for one slot the last is stored.  Results do not depend on any order of execution.
+ *
+ *   k, v [T, KVH, 128] bf16 or f32 (src_dtype); num_slots = NB * block_size
+ *   workspace     >= nvllm_b200_store_kvcache_q8_workspace_bytes(T) bytes, 16-byte aligned; need not be initialised
+ *                 (not used, and may be NULL, up to 1024 tokens)
+ */
+size_t nvllm_b200_store_kvcache_q8_workspace_bytes(int64_t T);
+int nvllm_b200_store_kvcache_q8(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scale,
+                                float* v_scale, const int32_t* slot_mapping, void* workspace, size_t workspace_bytes,
+                                int64_t T, int KVH, int D, int64_t num_slots, int src_dtype, void* stream);
+
+/*
+ * paged_decode_q8: nvllm_b200_paged_decode over an 8-bit cache; the arguments they share mean the same.
+ * Math: fp32 scores and softmax, fp16 probabilities into the P.V product with fp32 accumulation.
+ *
+ *   workspace     >= nvllm_b200_paged_decode_q8_workspace_bytes(B, H, KVH) bytes, 256-byte aligned; need not be initialised
+ */
+size_t nvllm_b200_paged_decode_q8_workspace_bytes(int B, int H, int KVH);
+int nvllm_b200_paged_decode_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                               const float* v_scale, const int32_t* block_tables, const int32_t* context_lens, void* out,
+                               void* workspace, size_t workspace_bytes, int B, int H, int KVH, int D, int NB,
+                               int block_size, int MB, float scale, void* stream);
+
+/*
+ * decode_step_q8: nvllm_b200_store_kvcache_q8 (T = B) followed by nvllm_b200_paged_decode_q8, as one C call and two launches
+ * (four beyond 1024 sequences): a decode step of the attention layer (layers/attention.py:436-480) over an 8-bit cache.
+ * Same workspace size as nvllm_b200_paged_decode_q8.
+ */
+int nvllm_b200_decode_step_q8(const void* q, const void* k, const void* v, void* k_cache, void* v_cache, float* k_scale,
+                              float* v_scale, const int32_t* slot_mapping, const int32_t* block_tables,
+                              const int32_t* context_lens, void* out, void* workspace, size_t workspace_bytes, int B, int H,
+                              int KVH, int D, int NB, int block_size, int MB, float scale, int src_dtype, void* stream);
+
+/*
+ * copy_pages: page src[i] of every cache -> page dst[i], i = 0 .. n-1, for a fork (a child's copy of a partly filled page)
+ * or a compaction (pages moved to free ones, with their block tables).  The reference shares whole pages by reference count
+ * (engine/block_manager.py:137-182) and has no counterpart.
+ *
+ *   caches_host   HOST array of num_caches device pointers: K, V and scale tensors of any layers, each NB pages
+ *   page_rows_host, row_bytes_host  HOST arrays: rows of a page (a divisor of block_size: block_size for K and V,
+ *                 block_size / 64 for scales) and bytes of a row (a multiple of 4) of every cache
+ *   src, dst      [n] int32; a pair with a page outside 0 .. NB-1 is skipped
+ *   tokens        [n] int32 or NULL: only the rows of the first tokens[i] tokens are copied (0 .. block_size); the other
+ *                 rows of the destination stay as they are
+ *   block_tables  int32, table_entries of them, or NULL: every entry that names a source is set to its destination (the
+ *                 first such pair's)
+ *
+ * Pairs are independent: the pages read hold what they held before the call.  A pair whose destination another pair reads
+ * from, or a later pair writes to, is left out (its table entries stay, too), and bit 7 (128) of the device status is raised.
+ */
+int nvllm_b200_copy_pages(void* const* caches_host, const int32_t* page_rows_host, const int64_t* row_bytes_host,
+                          int num_caches, const int32_t* src, const int32_t* dst, const int32_t* tokens, int n, int64_t NB,
+                          int block_size, int32_t* block_tables, int64_t table_entries, void* stream);
 
 /*
  * Clears the device-side error flags of the current device (see

@@ -43,6 +43,12 @@ SIGNATURES = {
     "nvllm_b200_allreduce_sum_emulated": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _sz, _c.c_uint, _i64, _vp]),
     "nvllm_b200_qk_norm_rope_store": (_i32, [_vp] * 10 + [_i64, _i32, _i32, _i32, _i64, _i64, _f32, _vp]),
     "nvllm_b200_fused_decode_step": (_i32, [_vp] * 7 + [_i64, _f32] + [_vp] * 7 + [_sz] + [_i32] * 7 + [_f32, _vp]),
+    "nvllm_b200_store_kvcache_q8_workspace_bytes": (_sz, [_i64]),
+    "nvllm_b200_store_kvcache_q8": (_i32, [_vp] * 8 + [_sz, _i64, _i32, _i32, _i64, _i32, _vp]),
+    "nvllm_b200_paged_decode_q8_workspace_bytes": (_sz, [_i32] * 3),
+    "nvllm_b200_paged_decode_q8": (_i32, [_vp] * 9 + [_sz] + [_i32] * 7 + [_f32, _vp]),
+    "nvllm_b200_decode_step_q8": (_i32, [_vp] * 12 + [_sz] + [_i32] * 7 + [_f32, _i32, _vp]),
+    "nvllm_b200_copy_pages": (_i32, [_vp] * 3 + [_i32] + [_vp] * 3 + [_i32, _i64, _i32, _vp, _i64, _vp]),
 }
 
 _lock = threading.Lock()

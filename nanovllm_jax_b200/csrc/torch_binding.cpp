@@ -34,6 +34,12 @@ struct Api {
     decltype(&nvllm_b200_prefill_step) prefill_step;
     decltype(&nvllm_b200_qk_norm_rope_store) qk_norm_rope_store;
     decltype(&nvllm_b200_fused_decode_step) fused_decode_step;
+    decltype(&nvllm_b200_store_kvcache_q8_workspace_bytes) store_q8_workspace_bytes;
+    decltype(&nvllm_b200_store_kvcache_q8) store_kvcache_q8;
+    decltype(&nvllm_b200_paged_decode_q8_workspace_bytes) decode_q8_workspace_bytes;
+    decltype(&nvllm_b200_paged_decode_q8) paged_decode_q8;
+    decltype(&nvllm_b200_decode_step_q8) decode_step_q8;
+    decltype(&nvllm_b200_copy_pages) copy_pages;
 } api = {};
 PyObject* check_fn = nullptr;  // raises NvllmError for a non-zero status, from the library's thread-local text
 
@@ -55,6 +61,7 @@ const char* dtype_text(at::ScalarType t) {
         case at::kBFloat16: return "torch.bfloat16";
         case at::kFloat: return "torch.float32";
         case at::kInt: return "torch.int32";
+        case at::kFloat8_e4m3fn: return "torch.float8_e4m3fn";
         default: return c10::toString(t);
     }
 }
@@ -578,6 +585,174 @@ PyObject* fused_decode_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// ---- the 8-bit cache -----------------------------------------------------------------------------------------------
+
+constexpr int kGrain = 64;  // slots of a scale
+
+// k_cache, v_cache [NB, block, KVH, 128] e4m3 and k_scale, v_scale [NB, block / 64, KVH] fp32 at a[0..3]
+struct Cache8 : Cache {
+    const at::Tensor &k, &v, &k_scale, &v_scale;
+};
+Cache8 cache8(PyObject* const* a) {
+    const at::Tensor& k = need(a[0], "k_cache", at::kFloat8_e4m3fn, 4);
+    const at::Tensor& v = need(a[1], "v_cache", at::kFloat8_e4m3fn, 4);
+    const at::Tensor& ks = need(a[2], "k_scale", at::kFloat, 3);
+    const at::Tensor& vs = need(a[3], "v_scale", at::kFloat, 3);
+    const int64_t nb = k.size(0), blk = k.size(1), kvh = k.size(2), d = k.size(3);
+    if (v.sizes() != k.sizes()) raise(PyExc_ValueError, "k_cache " + shape_text(k) + " and v_cache " + shape_text(v) + " differ");
+    if (blk % kGrain) raise(PyExc_ValueError, "the page size " + std::to_string(blk) + " must be a multiple of " + std::to_string(kGrain));
+    if (ks.sizes() != vs.sizes() || ks.size(0) != nb || ks.size(1) != blk / kGrain || ks.size(2) != kvh)
+        raise(PyExc_ValueError, "k_scale / v_scale must be (" + std::to_string(nb) + ", " + std::to_string(blk / kGrain) + ", " +
+                                    std::to_string(kvh) + "), got " + shape_text(ks) + " / " + shape_text(vs));
+    return Cache8{{nb * blk, (int)nb, (int)blk, (int)kvh, (int)d}, k, v, ks, vs};
+}
+void same_device(const at::Tensor& at, std::initializer_list<const at::Tensor*> others) {
+    for (const at::Tensor* t : others)
+        if (t->device() != at.device())
+            raise(PyExc_ValueError, "tensors on " + at.device().str() + " and on " + t->device().str());
+}
+void fits_q(const Cache8& c, const at::Tensor& q, int block_size) {
+    if (c.d != q.size(2) || c.block != block_size)
+        raise(PyExc_ValueError, "cache shape " + shape_text(c.k) + " inconsistent with q " + shape_text(q) + " / block " +
+                                    std::to_string(block_size));
+}
+
+// store_kvcache_q8(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+PyObject* store_kvcache_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return entry("store_kvcache_q8", n, 7, [&]() -> PyObject* {
+        const at::Tensor& key = tensor(a[0], "key");
+        const int src = source_dtype(key);
+        need(key, "key", key.scalar_type(), 3);
+        const at::Tensor& value = need(a[1], "value", key.scalar_type(), 3);
+        const Cache8 c = cache8(a + 2);
+        const at::Tensor& slots = need(a[6], "slot_mapping", at::kInt, 1);
+        same_device(key, {&value, &c.k, &c.v, &c.k_scale, &c.v_scale, &slots});
+        const int64_t t = key.size(0);
+        if (value.sizes() != key.sizes()) raise(PyExc_ValueError, "key and value shapes differ");
+        if (key.size(1) != c.kvh || key.size(2) != c.d)
+            raise(PyExc_ValueError, "key shape " + shape_text(key) + " inconsistent with cache " + shape_text(c.k));
+        if (slots.size(0) != t)
+            raise(PyExc_ValueError, "slot_mapping has " + std::to_string(slots.size(0)) + " entries for " + std::to_string(t) +
+                                        " tokens");
+        const Site site(key);
+        const at::Tensor ws = site.scratch(api.store_q8_workspace_bytes(t));
+        call([&] {
+            return api.store_kvcache_q8(ptr(key), ptr(value), mptr(c.k), mptr(c.v), (float*)mptr(c.k_scale), (float*)mptr(c.v_scale),
+                                        iptr(slots), mptr(ws), ws.nbytes(), t, c.kvh, c.d, c.slots, src, site.stream);
+        });
+        Py_RETURN_NONE;
+    });
+}
+
+// paged_decode_q8(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, scale, block_size, out)
+PyObject* paged_decode_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return entry("paged_decode_q8", n, 10, [&]() -> PyObject* {
+        const at::Tensor& q = need(a[0], "q", at::kBFloat16, 3);
+        const Cache8 c = cache8(a + 1);
+        const at::Tensor& bt = need(a[5], "block_tables", at::kInt, 2);
+        const at::Tensor& cl = need(a[6], "context_lens", at::kInt, 1);
+        const float scale = to_float(a[7]);
+        fits_q(c, q, to_int(a[8]));
+        same_device(q, {&c.k, &c.v, &c.k_scale, &c.v_scale, &bt, &cl});
+        const int b = (int)q.size(0), h = (int)q.size(1), mb = (int)bt.size(1);
+        if (bt.size(0) != b || cl.size(0) != b) raise(PyExc_ValueError, "block_tables / context_lens batch mismatch");
+        const Site site(q);
+        const at::Tensor out = output_like(a[9], q);
+        same_device(q, {&out});
+        const at::Tensor ws = site.scratch(api.decode_q8_workspace_bytes(b, h, c.kvh));
+        call([&] {
+            return api.paged_decode_q8(ptr(q), ptr(c.k), ptr(c.v), fptr(c.k_scale), fptr(c.v_scale), iptr(bt), iptr(cl), mptr(out),
+                                       mptr(ws), ws.nbytes(), b, h, c.kvh, c.d, c.nb, c.block, mb, scale, site.stream);
+        });
+        return result(a[9], out);
+    });
+}
+
+// decode_step_q8(q, key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables, context_lens, scale, block_size,
+//                out, coerce); coerce as in decode_step
+PyObject* decode_step_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return entry("decode_step_q8", n, 14, [&]() -> PyObject* {
+        at::Tensor q = tensor(a[0], "q"), key = tensor(a[1], "key"), value = tensor(a[2], "value");
+        const Cache8 c = cache8(a + 3);
+        if (a[13] == Py_True) {
+            if (q.scalar_type() != at::kBFloat16) q = q.to(at::kBFloat16);
+            if (!q.is_contiguous()) q = q.contiguous();
+            if (!key.is_contiguous()) key = key.contiguous();
+            if (!value.is_contiguous()) value = value.contiguous();
+        }
+        const int src = source_dtype(key);
+        need(q, "q", at::kBFloat16, 3);
+        need(key, "key", key.scalar_type(), 3);
+        need(value, "value", key.scalar_type(), 3);
+        const at::Tensor& slots = need(a[7], "slot_mapping", at::kInt, 1);
+        const at::Tensor& bt = need(a[8], "block_tables", at::kInt, 2);
+        const at::Tensor& cl = need(a[9], "context_lens", at::kInt, 1);
+        const float scale = to_float(a[10]);
+        fits_q(c, q, to_int(a[11]));
+        same_device(q, {&key, &value, &c.k, &c.v, &c.k_scale, &c.v_scale, &slots, &bt, &cl});
+        const int b = (int)q.size(0), h = (int)q.size(1), mb = (int)bt.size(1);
+        if (key.size(0) != b || key.size(1) != c.kvh || key.size(2) != c.d || value.sizes() != key.sizes())
+            raise(PyExc_ValueError, "key/value must be [" + std::to_string(b) + ", " + std::to_string(c.kvh) + ", " +
+                                        std::to_string(c.d) + "], got " + shape_text(key) + " / " + shape_text(value));
+        if (bt.size(0) != b || cl.size(0) != b || slots.size(0) != b)
+            raise(PyExc_ValueError, "block_tables / context_lens / slot_mapping batch mismatch");
+        const Site site(q);
+        const at::Tensor out = output_like(a[12], q);
+        same_device(q, {&out});
+        const at::Tensor ws = site.scratch(api.decode_q8_workspace_bytes(b, h, c.kvh));
+        call([&] {
+            return api.decode_step_q8(ptr(q), ptr(key), ptr(value), mptr(c.k), mptr(c.v), (float*)mptr(c.k_scale),
+                                      (float*)mptr(c.v_scale), iptr(slots), iptr(bt), iptr(cl), mptr(out), mptr(ws), ws.nbytes(), b, h,
+                                      c.kvh, c.d, c.nb, c.block, mb, scale, src, site.stream);
+        });
+        return result(a[12], out);
+    });
+}
+
+// copy_pages(caches, src, dst, block_size, tokens, block_tables)
+PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+    return entry("copy_pages", n_args, 6, [&]() -> PyObject* {
+        const Owned list{PySequence_Fast(a[0], "caches must be a sequence of CUDA tensors")};
+        if (!list.o) throw Raised();
+        const Py_ssize_t count = PySequence_Fast_GET_SIZE(list.o);
+        if (count == 0) raise(PyExc_ValueError, "no caches");
+        const at::Tensor& src = need(a[1], "src", at::kInt, 1);
+        const at::Tensor& dst = need(a[2], "dst", at::kInt, 1);
+        const int block = to_int(a[3]);
+        if (block <= 0) raise(PyExc_ValueError, "block_size must be positive");
+        if (dst.size(0) != src.size(0)) raise(PyExc_ValueError, "src and dst lengths differ");
+        const at::Tensor* tokens = a[4] == Py_None ? nullptr : &need(a[4], "tokens", at::kInt, 1);
+        const at::Tensor* tables = a[5] == Py_None ? nullptr : &need(a[5], "block_tables", at::kInt, 2);
+        if (tokens && tokens->size(0) != src.size(0)) raise(PyExc_ValueError, "tokens and src lengths differ");
+        same_device(src, {&dst, tokens ? tokens : &dst, tables ? tables : &dst});
+        std::vector<void*> base(count);
+        std::vector<int32_t> rows(count);
+        std::vector<int64_t> row_bytes(count);
+        int64_t nb = 0;
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            const at::Tensor& t = tensor(PySequence_Fast_ITEMS(list.o)[i], "a cache");
+            if (!t.is_cuda()) raise(PyExc_TypeError, "a cache must be a CUDA tensor");
+            if (!t.is_contiguous()) raise(PyExc_ValueError, "a cache must be contiguous");
+            if (t.dim() < 2) raise(PyExc_ValueError, "a cache must have at least 2 dims, got shape " + shape_text(t));
+            if (i == 0) nb = t.size(0);
+            if (t.size(0) != nb) raise(PyExc_ValueError, "caches of " + std::to_string(nb) + " and of " + std::to_string(t.size(0)) + " pages");
+            if (t.size(1) <= 0 || t.size(1) > block || block % t.size(1))
+                raise(PyExc_ValueError, "a cache " + shape_text(t) + " does not fit pages of " + std::to_string(block) + " tokens");
+            same_device(src, {&t});
+            int64_t row = t.element_size();
+            for (int64_t k = 2; k < t.dim(); ++k) row *= t.size(k);
+            base[i] = mptr(t), rows[i] = (int32_t)t.size(1), row_bytes[i] = row;
+        }
+        const Site site(src);
+        call([&] {
+            return api.copy_pages(base.data(), rows.data(), row_bytes.data(), (int)count, iptr(src), iptr(dst),
+                                  tokens ? iptr(*tokens) : nullptr, (int)src.size(0), nb, block,
+                                  tables ? (int32_t*)mptr(*tables) : nullptr, tables ? tables->numel() : 0, site.stream);
+        });
+        Py_RETURN_NONE;
+    });
+}
+
 // workspace(device_index, nbytes): the scratch buffer of the device's current stream
 PyObject* py_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return entry("workspace", n, 2, [&]() -> PyObject* {
@@ -659,6 +834,12 @@ PyObject* bind(PyObject*, PyObject* args) {
         {"nvllm_b200_prefill_step", (void**)&api.prefill_step},
         {"nvllm_b200_qk_norm_rope_store", (void**)&api.qk_norm_rope_store},
         {"nvllm_b200_fused_decode_step", (void**)&api.fused_decode_step},
+        {"nvllm_b200_store_kvcache_q8_workspace_bytes", (void**)&api.store_q8_workspace_bytes},
+        {"nvllm_b200_store_kvcache_q8", (void**)&api.store_kvcache_q8},
+        {"nvllm_b200_paged_decode_q8_workspace_bytes", (void**)&api.decode_q8_workspace_bytes},
+        {"nvllm_b200_paged_decode_q8", (void**)&api.paged_decode_q8},
+        {"nvllm_b200_decode_step_q8", (void**)&api.decode_step_q8},
+        {"nvllm_b200_copy_pages", (void**)&api.copy_pages},
     };
     for (const auto& e : entries) {
         PyObject* addr = PyDict_GetItemString(table, e.name);
@@ -682,6 +863,10 @@ PyMethodDef methods[] = {
     FAST("prefill_step", prefill_step),
     FAST("qk_norm_rope_store", qk_norm_rope_store),
     FAST("fused_decode_step", fused_decode_step),
+    FAST("store_kvcache_q8", store_kvcache_q8),
+    FAST("paged_decode_q8", paged_decode_q8),
+    FAST("decode_step_q8", decode_step_q8),
+    FAST("copy_pages", copy_pages),
     FAST("workspace", py_workspace),
     FAST("fill_decode_metadata", fill_decode_metadata),
     {"bind", bind, METH_VARARGS, nullptr},

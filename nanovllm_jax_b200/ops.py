@@ -104,3 +104,48 @@ def fused_decode_step(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, q
     launches; returns the attention output [B, H, D]."""
     return _lib.binding().fused_decode_step(q, key, value, q_weight, k_weight, cos_sin_cache, positions, k_cache, v_cache,
                                             slot_mapping, block_tables, context_lens, scale, block_size, eps, out)
+
+
+def store_kvcache_q8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """In place: the rows into an 8-bit cache by slot, as ``store_kvcache`` does into a bf16 one.
+
+    key/value: [T, KVH, 128] bf16 or fp32.  Caches: float8_e4m3fn [NB, block, KVH, 128]; scales: fp32 [NB, block / 64, KVH],
+    one for every 64 slots and kv head (an element stands for value * scale).  The store chooses a power of two.  A call that
+    writes the first of 64 slots begins them anew; later ones may let their scale grow, which rounds the rows again that the 64
+    slots hold already.  slot_mapping: [T] int32; negative = skip.
+    """
+    _lib.binding().store_kvcache_q8(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+
+
+def paged_decode_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                    v_scale: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor, scale: float,
+                    block_size: int, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention over an 8-bit paged cache (see ``store_kvcache_q8``); returns [B, H, 128] bf16."""
+    return _lib.binding().paged_decode_q8(q, k_cache, v_cache, k_scale, v_scale, block_tables, context_lens, scale, block_size,
+                                          out)
+
+
+def decode_step_q8(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor, block_tables: torch.Tensor,
+                   context_lens: torch.Tensor, scale: float, block_size: int,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """One decode step of one layer over an 8-bit cache in one C call: same result as ``store_kvcache_q8`` followed by
+    ``paged_decode_q8``."""
+    return _lib.binding().decode_step_q8(q, key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, block_tables,
+                                         context_lens, scale, block_size, out, False)
+
+
+def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor, block_size: int, tokens: torch.Tensor | None = None,
+               block_tables: torch.Tensor | None = None) -> None:
+    """In place: ``cache[dst[i]] = cache[src[i]]`` for every pair i and every tensor of ``caches``, in one launch.
+
+    caches: a sequence of contiguous tensors [NB, rows, ...] of any layers and types: K and V caches (rows = block_size) and
+    their scales (rows = block_size / 64).  src/dst: [n] int32 page ids; a pair with an id outside 0 .. NB - 1 (padding) is
+    skipped.  tokens: [n] int32, copies only the rows of a page's first tokens (the fork of a partly filled page).
+    block_tables: [B, MB] int32, updated in place: entries that name a source name its destination afterwards (a move).
+
+    A destination may not be a source of another pair, nor occur twice: such a pair is left out (of two that write the same page
+    the later one is carried out) and bit 7 (128) of ``_lib.device_status()`` is raised.
+    """
+    _lib.binding().copy_pages(caches, src, dst, block_size, tokens, block_tables)
