@@ -345,7 +345,7 @@ int nvllm_b200_allreduce_sum_emulated(void* const* in, void* const* out, void* c
  * A cache in half the bytes: k_cache, v_cache hold e4m3 values [NB, block_size, KVH, 128] and k_scale, v_scale fp32 scales
  * [NB, block_size / 64, KVH], one for every 64 slots and kv head; an element stands for value * scale.  It has no
  * counterpart in the reference, whose cache is bf16 (engine/model_runner.py:176).  block_size is a multiple of 64.  The attention entry points take
- * any finite scales; those that the store writes are powers of two.
+ * any positive finite scales; those that the store writes are powers of two.
  *
  * store_kvcache_q8: nvllm_b200_store_kvcache (same slot rules) into an 8-bit cache.
  *
@@ -388,6 +388,19 @@ int nvllm_b200_decode_step_q8(const void* q, const void* k, const void* v, void*
                               float* v_scale, const int32_t* slot_mapping, const int32_t* block_tables,
                               const int32_t* context_lens, void* out, void* workspace, size_t workspace_bytes, int B, int H,
                               int KVH, int D, int NB, int block_size, int MB, float scale, int src_dtype, void* stream);
+
+/*
+ * paged_prefill_q8: nvllm_b200_paged_prefill over an 8-bit cache (block_size a multiple of 128); the arguments they share, the
+ * workspace and the device status bits mean the same.  The new tokens' rows must have been stored already.
+ * Math: scores in fp32 from the cache's own values and from q as the sum of two e4m3 numbers under a power of two per row (exact
+ * for components above 2^-11 of the row's largest, to within 2^-18 of it for smaller ones); bf16 probabilities and bf16
+ * value * scale (exact for scales that are powers of two) into the P.V product with fp32 accumulation.
+ */
+int nvllm_b200_paged_prefill_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                                const float* v_scale, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                const int32_t* block_tables, const int32_t* cu_seqlens_q_host, void* out, void* workspace,
+                                size_t workspace_bytes, int64_t T, int B, int max_seqlen_q, int H, int KVH, int D, int NB,
+                                int block_size, int MB, float scale, void* stream);
 
 /*
  * copy_pages: page src[i] of every cache -> page dst[i], i = 0 .. n-1, for a fork (a child's copy of a partly filled page)

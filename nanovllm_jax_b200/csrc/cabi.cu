@@ -57,13 +57,14 @@ extern "C" const char* nvllm_b200_last_error_string(void) { return nvllm::last_e
 extern "C" int nvllm_b200_device_status(int* flags_host) {
     using namespace nvllm;
     if (!flags_host) return fail(NVLLM_B200_EINVAL, "device_status: null pointer");
-    int a = 0, b = 0, c = 0, d = 0, e = 0, rc;
+    int a = 0, b = 0, c = 0, d = 0, e = 0, f = 0, rc;
     if ((rc = read_decode_flags(&a))) return rc;
     if ((rc = read_prefill_flags(&b))) return rc;
     if ((rc = read_comm_flags(&c))) return rc;
     if ((rc = read_decode_q8_flags(&d))) return rc;
     if ((rc = read_pages_flags(&e))) return rc;
-    *flags_host = a | b | c | d | e;
+    if ((rc = read_prefill_q8_flags(&f))) return rc;
+    *flags_host = a | b | c | d | e | f;
     return NVLLM_B200_OK;
 }
 
@@ -74,5 +75,6 @@ extern "C" int nvllm_b200_device_status_reset(void) {
     if ((rc = clear_prefill_flags())) return rc;
     if ((rc = clear_decode_q8_flags())) return rc;
     if ((rc = clear_pages_flags())) return rc;
+    if ((rc = clear_prefill_q8_flags())) return rc;
     return clear_comm_flags();
 }

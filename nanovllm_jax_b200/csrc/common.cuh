@@ -49,8 +49,10 @@ int clear_decode_flags();
 int clear_prefill_flags();
 int clear_comm_flags();
 int read_decode_q8_flags(int* out);
+int read_prefill_q8_flags(int* out);
 int read_pages_flags(int* out);
 int clear_decode_q8_flags();
+int clear_prefill_q8_flags();
 int clear_pages_flags();
 
 // Programmatic dependent launch between the library's kernels is on unless NVLLM_B200_PDL=0.

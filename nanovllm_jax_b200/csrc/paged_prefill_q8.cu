@@ -1,0 +1,801 @@
+// paged_prefill_q8: causal attention of new tokens over their whole sequences in the 8-bit paged cache, on the sm_100a tensor
+// cores.
+//
+// Work items, tiles, runs and the softmax warps are those of the bf16 kernel (varlen_prefill.cu, and see there); what differs is
+// how bytes become operands.  Converting a whole K/V tile to bf16 in the SM would double what goes through its shared memory,
+// which the two products fill to nine tenths already, so as little as possible is converted:
+//
+//  * Q.K^T takes K as it is, e4m3 from TMA (tcgen05.mma kind::f8f6f4, K = 32 per instruction), and Q as the sum of two e4m3 tiles.
+//    bf16 has eight significant bits, e4m3 four: with a row divided by the power of two that brings its largest magnitude to
+//    224 .. 448, hi = e4m3(q) and lo = e4m3(q - hi) give every q above 2^-11 of that exactly, and a smaller one to within 2^-18 of
+//    it.  Twice as many products at twice the rate: the time of the bf16 product, with no conversion of K at all.
+//  * The row's power of two and the K scale of each half of a tile (a scale has 64 slots) go into the factor that the softmax
+//    multiplies its scores by anyway.
+//  * O += P.V stays in bf16: P would lose its small probabilities in e4m3.  A warpgroup of its own turns V bytes into bf16
+//    (value * scale: exact where the scale is a power of two, as the store's are) with rows behind the sequence's end as zeros,
+//    one tile ahead, and splits Q between two items.
+//
+// Per CTA (16 warps = 4 warpgroups; registers 64 | 184 | 184 | 80 of the launch's 128 each):
+//   warp 0       TMA producer: K and V bytes, three slots each; the scales of a tile, fetched a tile ahead, into a ring
+//   warps 1, 2   MMA issuers of Q tiles A and B
+//   warp 3       item records
+//   warps 4-11   softmax, as in the bf16 kernel
+//   warps 12-15  Q: bf16 -> two e4m3 tiles and the rows' factors.  V: e4m3 -> bf16, two slots
+// Every mbarrier wait is bounded; on timeout the CTA raises a device error flag, lets its copies land and releases its
+// tensor memory before it exits.
+#include "q8.cuh"
+#include "varlen_prefill.cuh"
+
+#include <mutex>
+#include <type_traits>
+
+namespace nvllm {
+namespace prefill_q8 {
+
+using namespace prefill;
+
+__device__ int g_error_flag = 0;  // bit 2 (4): a pipeline wait timed out, or no room in tensor memory
+
+constexpr int kThreads = 512;
+constexpr int kByteTile = 128 * 128;     // 128 rows of 128 bytes, 128B-swizzled
+constexpr int kSlots = 3;                // of K bytes, and of V bytes
+constexpr int kVSlots = 2;               // of V in bf16
+constexpr int kScales = 8;               // ring of tile scales: nobody is as far ahead of a reader (see the producer)
+constexpr int kK = 2 * kTileBytes;       // offsets: Q (A: hi, lo; B: hi, lo), K, V bytes, V
+constexpr int kVBytes = kK + kSlots * kByteTile;
+constexpr int kV = kVBytes + kSlots * kByteTile;
+constexpr int kSmemTiles = kV + kVSlots * kTileBytes;  // 224 KB
+constexpr int kItemRing = 2;
+constexpr int kItemReaders = 3 + 8 + 4;  // TMA producer, two MMA issuers, eight softmax warps, four converting warps
+constexpr int kRegsControl = 64, kRegsSoftmax = 184, kRegsConvert = 80;
+static_assert(kRegsControl + 2 * kRegsSoftmax + kRegsConvert == 4 * 128, "what setmaxnreg asks for is what the launch has");
+
+constexpr float kTiny = 1.17549435e-38f;
+
+struct Source {
+    const __nv_bfloat16* q;
+    const float *k_scale, *v_scale;  // [NB * block_size / 64, KVH]
+    int NB, KVH;
+};
+struct Whole : Params {
+    Source in;
+};
+struct Split : SplitParams {
+    Source in;
+};
+
+struct Shared {
+    float q_factor[2][2][kTileQ];  // [item parity][Q tile][row]: what a row was divided by
+    float4 scale[kScales];         // of a tile: K first and second half, V first and second half
+    Item items[kItemRing];         // the items of this CTA, written ahead by warp 3
+    uint64_t item_full[kItemRing], item_empty[kItemRing];
+    uint64_t q_full, q_empty;
+    uint64_t factor_full[2];       // of the item parity: the softmax may come to an item when Q of the next one is there already
+    uint64_t k_full[kSlots], k_empty[kSlots];
+    uint64_t vb_full[kSlots], vb_empty[kSlots];  // V bytes
+    uint64_t v_full[kVSlots], v_empty[kVSlots];
+    uint64_t scale_full[kScales];
+    uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
+    uint64_t turn[2];  // as in the bf16 kernel
+    uint32_t tmem_base;
+    volatile int abort_flag;
+};
+constexpr int kSmemBytes = kSmemTiles + sizeof(Shared);
+static_assert(kSmemBytes <= 227 * 1024, "shared memory of a CTA");
+
+__device__ __forceinline__ bool wait_or_abort(Shared* sh, uint64_t* bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (sh->abort_flag) return false;
+    if (mbar_wait(bar, parity)) return true;
+    sh->abort_flag = 1;
+    atomicOr(&g_error_flag, 4);
+    return false;
+}
+
+__device__ __forceinline__ bool next_item(Shared* sh, uint32_t k, Item& it) {
+    const uint32_t slot = k % kItemRing;
+    if (!wait_or_abort(sh, &sh->item_full[slot], (k / kItemRing) & 1u)) return false;
+    it = sh->items[slot];
+    return it.n_kv >= 0;
+}
+
+// D[tmem] (+)= A[smem] * B[smem], both e4m3, K = 32
+__device__ __forceinline__ void mma_bytes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+constexpr uint32_t kIdescBytes = (1u << 4) | ((128u >> 4) << 24);  // e4m3 x e4m3 -> fp32, M = 128, both K-major
+constexpr uint32_t idesc_bytes(uint32_t keys) { return kIdescBytes | ((keys >> 3) << 17); }
+
+// One 128-column S row -> running max, optional O rescale, bf16 P in two halves.  DIAG: key column c of this tile is
+// visible iff c <= lim (lim may be negative -- nothing visible in this tile -- or >= 127), and the limits of the warp's rows
+// lie in warp_lo .. warp_hi; columns behind every limit may hold anything.  alive: the warp's rows in front of the
+// sequence's end; the others (the next sequence's queries, rows that no load fills) have no vote on when to rescale, or the
+// live rows' bits would depend on them.  turn_bar (or null): the other tile's hand-over this tile's exponentials wait for;
+// turn_out (or null): where this tile hands over.
+// The whole row is held in registers (the softmax warpgroups raise their register budget with setmaxnreg), so
+// tensor memory is read once and its latency is paid once per tile.
+template <bool DIAG>
+__device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint32_t t_s, const uint32_t t_o,
+                                             const int lim, const int warp_lo, const int warp_hi, const bool first,
+                                             const uint32_t o_parity_prev,
+                                             const float c0, const float c1, const uint32_t alive, float& m_run, float& m_used, float& l,
+                                             uint64_t* turn_bar, const uint32_t turn_parity, uint64_t* turn_out) {
+    uint32_t v[4][32];
+    tmem_ld32(t_s, v[0]);
+    tmem_ld32(t_s + 32, v[1]);
+    tmem_ld32(t_s + 64, v[2]);
+    tmem_ld32(t_s + 96, v[3]);
+    tmem_wait_ld();
+    float top[2] = {-INFINITY, -INFINITY};  // of the two halves
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if (DIAG) {
+            if (32 * c > warp_hi) continue;  // nothing of this chunk is visible to any row of the warp
+            if (32 * c + 31 > warp_lo) {     // mask in place so that the second pass needs no select
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (c * 32 + i > lim) v[c][i] = 0xFF800000u;
+            }
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            mx0 = max3(mx0, __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+            mx1 = max3(mx1, __uint_as_float(v[c][i + 2]), __uint_as_float(v[c][i + 3]));
+            mx2 = max3(mx2, __uint_as_float(v[c][i + 4]), __uint_as_float(v[c][i + 5]));
+            mx3 = max3(mx3, __uint_as_float(v[c][i + 6]), __uint_as_float(v[c][i + 7]));
+        }
+        top[c >> 1] = max3(top[c >> 1], fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+    }
+    m_run = max3(m_run, top[0] * c0, top[1] * c1);
+    if (turn_bar != nullptr && !wait_or_abort(sh, turn_bar, turn_parity)) return false;
+    if (first) {
+        m_used = m_run;  // finite for live rows: key 0 of the sequence is visible to every row and sits in the first tile
+    } else {
+        const bool grow = m_run - m_used > kRescaleThreshold;
+        if (__ballot_sync(0xffffffffu, grow) & alive) {
+            // O holds sums relative to m_used: bring it to m_run before this tile's P.V is added.
+            if (!wait_or_abort(sh, &sh->o_full[x], o_parity_prev)) return false;
+            tc_fence_after();
+            const float f = fast_exp2(m_used - m_run);
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                uint32_t ov[16];
+                tmem_ld16(t_o + c * 16, ov);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+                tmem_st16(t_o + c * 16, ov);
+            }
+            tmem_wait_st();
+            l *= f;
+            m_used = m_run;
+        }
+    }
+    // p = 2^(s*scale - m) as bf16 pairs, written over the S columns (all of them are in registers by now):
+    // chunk c (scores 32c..32c+31) becomes packed columns 16c..16c+15.
+    const uint64_t neg2 = pack2(-m_used, -m_used);
+    uint64_t acc_a = pack2(0.f, 0.f), acc_b = pack2(0.f, 0.f);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        if (DIAG && 32 * c > warp_hi) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[c][i] = 0u;
+        } else {
+        const uint64_t scale2 = c < 2 ? pack2(c0, c0) : pack2(c1, c1);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            float x0, x1, x2, x3;
+            unpack2(fma2(pack2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), scale2, neg2), x0, x1);
+            unpack2(fma2(pack2(__uint_as_float(v[c][2 * i + 2]), __uint_as_float(v[c][2 * i + 3])), scale2, neg2), x2,
+                    x3);
+            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);  // 2^-inf = 0 for masked keys
+            const float e2 = fast_exp2(x2), e3 = fast_exp2(x3);
+            acc_a = add2(acc_a, pack2(e0, e1));
+            acc_b = add2(acc_b, pack2(e2, e3));
+            v[c][i] = pack_bf16(e0, e1);  // in place: word i <= 2i has been consumed
+            v[c][i + 1] = pack_bf16(e2, e3);
+        }
+        }
+        tmem_st16(t_s + c * 16, v[c]);
+        if (c == 3 && turn_out != nullptr) {
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(turn_out);
+        }
+        if (c & 1) {  // a half of P (64 keys) is complete: release its four P.V k-steps
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->p_full[x][c >> 1]);
+        }
+    }
+    float s0, s1, s2, s3;
+    unpack2(acc_a, s0, s1);
+    unpack2(acc_b, s2, s3);
+    l += (s0 + s1) + (s2 + s3);
+    return true;
+}
+
+template <class P>
+__global__ void __launch_bounds__(kThreads, 1)
+paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                        const __grid_constant__ P p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Shared* sh = reinterpret_cast<Shared*>(smem + kSmemTiles);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (smem_u32(smem) & 1023) {  // the swizzled tiles need it; the alignment above asks for it
+        if (tid == 0) atomicOr(&g_error_flag, 4);
+        griddep_wait();
+        return;
+    }
+    if (tid == 0) {
+        for (int s = 0; s < kItemRing; ++s) {
+            mbar_init(&sh->item_full[s], 1);
+            mbar_init(&sh->item_empty[s], kItemReaders);
+        }
+        mbar_init(&sh->q_full, 4);    // the converting warps
+        mbar_init(&sh->q_empty, 2);   // both MMA issuers
+        mbar_init(&sh->factor_full[0], 4);
+        mbar_init(&sh->factor_full[1], 4);
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(&sh->k_full[s], 1);
+            mbar_init(&sh->k_empty[s], 2);
+            mbar_init(&sh->vb_full[s], 1);
+            mbar_init(&sh->vb_empty[s], 4);
+        }
+        for (int s = 0; s < kVSlots; ++s) {
+            mbar_init(&sh->v_full[s], 4);
+            mbar_init(&sh->v_empty[s], 2);
+        }
+        for (int s = 0; s < kScales; ++s) mbar_init(&sh->scale_full[s], 1);
+        for (int x = 0; x < 2; ++x) {
+            mbar_init(&sh->s_full[x], 1);
+            mbar_init(&sh->p_full[x][0], kTileQ / 32);
+            mbar_init(&sh->p_full[x][1], kTileQ / 32);
+            mbar_init(&sh->o_full[x], 1);
+            mbar_init(&sh->o_empty[x], kTileQ / 32);
+            mbar_init(&sh->turn[x], kTileQ / 32);
+        }
+        sh->abort_flag = 0;
+        sh->tmem_base = 0xFFFFFFFFu;
+        fence_mbar_init();
+        prefetch_tensormap(&tm_k);
+        prefetch_tensormap(&tm_v);
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tmem_alloc(&sh->tmem_base, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem_base;
+
+    griddep_wait();  // the plan kernel's item list (and the caller's q and cache) must be visible from here on
+
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+    if (warp == 0) {
+        // =============================== TMA producer ===============================
+        if (lane == 0) {
+            uint32_t t = 0, i = 0;  // tiles, items
+            bool ok = true;
+            Item it = {};
+            int token = 0;
+            float4 scale;
+            // First slot of K/V tile j and its scales: one per 64 slots, of which the second may lie behind the last key.
+            auto locate = [&](int j) {
+                const int off = (max(it.kv0, 0) + j) * kTileKV;
+                const int page = __ldg(p.block_tables + (size_t)it.b * p.MB + min(off / p.block_size, p.MB - 1));
+                token = min(max(page, 0), p.in.NB - 1) * p.block_size + off % p.block_size;
+                const size_t at = (size_t)(token / q8::kGrain) * p.in.KVH + it.kvh;
+                const bool second = it.len_k - j * kTileKV > q8::kGrain;
+                scale.x = __ldg(p.in.k_scale + at);
+                scale.y = second ? __ldg(p.in.k_scale + at + p.in.KVH) : 1.f;
+                scale.z = __ldg(p.in.v_scale + at);
+                scale.w = second ? __ldg(p.in.v_scale + at + p.in.KVH) : 1.f;
+            };
+            while (ok && next_item(sh, i, it)) {
+                mbar_arrive(&sh->item_empty[i % kItemRing]);
+                locate(0);
+                for (int j = 0; j < it.n_kv; ++j, ++t) {
+                    const int slot = t % kSlots, here = token;
+                    const uint32_t empty = ((t / kSlots) & 1u) ^ 1u;
+                    const float4 mine = scale;
+                    if (j + 1 < it.n_kv) locate(j + 1);
+                    if (!(ok = wait_or_abort(sh, &sh->k_empty[slot], empty))) break;
+                    // Q.K^T(t - 3) is complete, so P.V(t - 4) has been issued: softmax and conversion have read the scales
+                    // of tile t - 4, and those of t - 8 are free to go.
+                    sh->scale[t % kScales] = mine;
+                    mbar_arrive(&sh->scale_full[t % kScales]);
+                    mbar_expect_tx(&sh->k_full[slot], kByteTile);
+                    tma_load_3d(smem + kK + slot * kByteTile, &tm_k, &sh->k_full[slot], 0, it.kvh, here);
+                    if (!(ok = wait_or_abort(sh, &sh->vb_empty[slot], empty))) {
+                        (void)mbar_wait(&sh->k_full[slot], (t / kSlots) & 1u, polls_of_ms(90));
+                        break;
+                    }
+                    mbar_expect_tx(&sh->vb_full[slot], kByteTile);
+                    tma_load_3d(smem + kVBytes + slot * kByteTile, &tm_v, &sh->vb_full[slot], 0, it.kvh, here);
+                }
+                ++i;
+            }
+            if (sh->abort_flag)  // loads in flight land before the memory is released
+                for (uint32_t u = t >= kSlots ? t - kSlots : 0; u < t; ++u) {
+                    (void)mbar_wait(&sh->k_full[u % kSlots], (u / kSlots) & 1u, polls_of_ms(90));
+                    (void)mbar_wait(&sh->vb_full[u % kSlots], (u / kSlots) & 1u, polls_of_ms(90));
+                }
+        }
+    } else if (warp == 3) {
+        // ============================== item records ================================
+        if (lane == 0) {
+            const List list = list_of(p);
+            const int total = tmem != 0xFFFFFFFFu ? items_of(p, list) : 0;
+            uint32_t k = 0;
+            int idx = blockIdx.x;
+            while (true) {
+                const uint32_t slot = k % kItemRing;
+                if (!wait_or_abort(sh, &sh->item_empty[slot], ((k / kItemRing) & 1u) ^ 1u)) break;
+                Item it;
+                do {
+                    if (k > 0 || idx != (int)blockIdx.x) idx = claim_item(p);
+                    it.n_kv = -1;
+                    if (idx < total) it = load_item(p, list, idx);
+                    if (it.n_kv == 0) idx = total;  // nothing to do there: claim another one
+                } while (it.n_kv == 0);
+                sh->items[slot] = it;
+                mbar_arrive(&sh->item_full[slot]);
+                if (it.n_kv < 0) break;
+                ++k;
+            }
+        }
+    } else {
+        // ============================== MMA issuers ===============================
+        // As in the bf16 kernel: one issuing thread per Q tile, K(j+1) awaited before P.V(j) is issued, all commits of the
+        // pair behind Q.K^T(j+1); a tile's last products leave out the keys behind every row.
+        if (lane == 0) {
+            const int x = warp - 1;
+            const uint32_t s_t = tmem + x * 128, o_t = tmem + 256 + x * 128;
+            const uint64_t q_desc = make_desc(smem_u32(smem + x * kTileBytes), 16, 1024);
+            const uint64_t k_desc0 = make_desc(smem_u32(smem + kK), 16, 1024), v_desc0 = mnmajor_desc(smem_u32(smem + kV), 0);
+            uint32_t kt = 0;     // K/V tiles consumed before this item
+            uint32_t tiles = 0;  // tiles finished by this Q tile, over all items (barrier phases)
+            uint32_t used = 0;   // items in which this Q tile was active (o_empty phases)
+            uint32_t i = 0;      // items
+            bool ok = true;
+
+            auto issue_qk = [&](uint64_t kd, bool behind_pv, uint32_t idesc) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half)  // the two tiles that Q is the sum of
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        mma_bytes(s_t, q_desc + (uint32_t)((half * kByteTile + ks * 32) >> 4), kd + (uint32_t)((ks * 32) >> 4), idesc,
+                                  half + ks > 0);
+                if (behind_pv) tc_commit(&sh->o_full[x]);
+                tc_commit(&sh->s_full[x]);
+            };
+            auto issue_pv = [&](int j, uint64_t vd, auto last, int steps) -> bool {
+                if (j == 0 && used > 0 && !wait_or_abort(sh, &sh->o_empty[x], (used - 1) & 1u)) return false;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (!wait_or_abort(sh, &sh->p_full[x][half], tiles & 1u)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = half * 4; ks < half * 4 + 4; ++ks)
+                        if (!decltype(last)::value || ks < steps)
+                            mma_ts(o_t, s_t + ks * 8, vd + (uint32_t)((ks * 16 * 128) >> 4), kIdescPV, (j > 0 || ks > 0));
+                }
+                ++tiles;
+                return true;
+            };
+            auto k_full = [&](uint32_t t) { return wait_or_abort(sh, &sh->k_full[t % kSlots], (t / kSlots) & 1u); };
+            auto k_desc = [&](uint32_t t) { return k_desc0 + (t % kSlots) * (uint32_t)(kByteTile >> 4); };
+
+            const std::false_type full;
+            const std::true_type last;
+            Item it;
+            while (ok && next_item(sh, i, it)) {
+                mbar_arrive(&sh->item_empty[i % kItemRing]);
+                const int n_x = x == 0 ? it.n_a : it.n_b;
+                const int steps = key_steps(visible_keys(p, it, x), n_x);  // of the last tile
+                const uint32_t idesc_last = idesc_bytes(16 * steps);
+                if (!(ok = wait_or_abort(sh, &sh->q_full, i & 1u))) break;
+                if (n_x == 0) mbar_arrive(&sh->q_empty);  // this tile never reads the Q buffer of this item
+                if (!(ok = k_full(kt))) break;
+                if (n_x > 0) {
+                    tc_fence_after();
+                    issue_qk(k_desc(kt), false, n_x > 1 ? idesc_bytes(kTileKV) : idesc_last);
+                    tc_commit(&sh->k_empty[kt % kSlots]);
+                    if (n_x == 1) tc_commit(&sh->q_empty);
+                } else {
+                    mbar_arrive(&sh->k_empty[kt % kSlots]);
+                }
+                for (int j = 0; ok && j < it.n_kv; ++j) {
+                    const uint32_t t = kt + j, vs = t % kVSlots;
+                    if (!(ok = wait_or_abort(sh, &sh->v_full[vs], (t / kVSlots) & 1u))) break;
+                    if (j + 1 < it.n_kv && !(ok = k_full(t + 1))) break;
+                    if (j < n_x) {
+                        const uint64_t vd = v_desc0 + vs * (uint32_t)(kTileBytes >> 4);
+                        if (j + 1 < n_x) {
+                            if (!(ok = issue_pv(j, vd, full, 8))) break;
+                        } else {
+                            if (!(ok = issue_pv(j, vd, last, steps))) break;
+                            tc_commit(&sh->o_full[x]);
+                            tc_commit(&sh->v_empty[vs]);
+                        }
+                    } else {
+                        mbar_arrive(&sh->v_empty[vs]);
+                    }
+                    if (j + 1 < it.n_kv) {
+                        if (j + 1 < n_x) {
+                            issue_qk(k_desc(t + 1), true, j + 2 < n_x ? idesc_bytes(kTileKV) : idesc_last);
+                            tc_commit(&sh->k_empty[(t + 1) % kSlots]);
+                            tc_commit(&sh->v_empty[vs]);
+                            if (j + 2 == n_x) tc_commit(&sh->q_empty);  // this tile's last Q.K^T has been issued
+                        } else {
+                            mbar_arrive(&sh->k_empty[(t + 1) % kSlots]);
+                        }
+                    }
+                }
+                used += n_x > 0 ? 1 : 0;
+                kt += it.n_kv;
+                ++i;
+            }
+        }
+    }
+    } else if (warp < 12) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        // ============================ softmax warpgroups ============================
+        const int x = (warp - 4) >> 2;              // 0: tile A, 1: tile B
+        const int quarter = warp & 3;               // tensor-memory lane quarter this warp may touch
+        const int row = quarter * 32 + lane;        // row within the Q tile: a token and a head
+        const int tok = row / p.pack.heads, tok_head = row - tok * p.pack.heads;
+        const int tok_lo = quarter * 32 / p.pack.heads, tok_hi = (quarter * 32 + 31) / p.pack.heads;  // the warp's tokens
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        const uint32_t t_s = tmem + x * 128 + lane_base;
+        const uint32_t t_o = tmem + 256 + x * 128 + lane_base;
+        uint32_t tiles = 0;  // tiles finished by this Q tile over all items (barrier phases)
+        uint32_t turns_seen = 0;  // completions of the other tile's turn barrier this warp has consumed
+        uint32_t kt = 0;          // K/V tiles of the items before this one
+        bool ok = true;
+        Item it;
+        for (uint32_t k = 0; ok && next_item(sh, k, it); ++k) {
+            const int n_x = x == 0 ? it.n_a : it.n_b;
+            const uint32_t kt0 = kt;
+            kt += it.n_kv;
+            if (n_x == 0) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->item_empty[k % kItemRing]);
+                continue;
+            }
+            // The two tiles take turns, as in the bf16 kernel.
+            const bool both = it.n_b > 0 && it.n_a > 1;
+            const int q_pos = it.q0 + x * p.pack.dq;      // first token of this Q tile
+            const int first_lim = it.prefix + q_pos;      // last key visible to it
+            const int live = min(p.pack.tokens, it.len - q_pos);  // tokens of the tile in front of the sequence's end
+            float m_run = -INFINITY, m_used = -INFINITY, l = 0.f;
+            if (!(ok = wait_or_abort(sh, &sh->factor_full[k & 1], (k >> 1) & 1u))) break;
+            const float factor = sh->q_factor[k & 1][x][row] * p.scale_log2;
+            const uint32_t alive = __ballot_sync(0xffffffffu, tok < live);
+            // One KV tile of this Q tile.  Tiles whose last key the tile's first row may still see need no mask; the
+            // one or two after them (one when the prefix is a multiple of the tile) are masked per element.  The two
+            // kinds run in two separate loops so that each loop body is straight-line code.
+            auto tile_step = [&](const int j, auto kind) -> bool {
+                constexpr bool kDiag = decltype(kind)::value == 1, kDead = decltype(kind)::value == 2;
+                if (!wait_or_abort(sh, &sh->s_full[x], tiles & 1u)) return false;
+                // A(j) starts after B(j-1); B(j) starts after A(j) while A still has tiles.
+                uint64_t* turn_bar = nullptr;
+                const uint32_t turn_parity = turns_seen & 1u;
+                if (both && (x == 0 ? j >= 1 : j < it.n_a)) {
+                    turn_bar = &sh->turn[x ^ 1];
+                    ++turns_seen;
+                }
+                tc_fence_after();
+                if constexpr (kDead) {  // nothing but the hand-overs: P and O of these rows may hold anything
+                    if (turn_bar != nullptr && !wait_or_abort(sh, turn_bar, turn_parity)) return false;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (both && (x == 0 || j < it.n_a)) mbar_arrive(&sh->turn[x]);
+                        mbar_arrive(&sh->p_full[x][0]);
+                        mbar_arrive(&sh->p_full[x][1]);
+                    }
+                    ++tiles;
+                    return true;
+                }
+                const int lim = first_lim - j * kTileKV;
+                const uint32_t t = kt0 + j;
+                if (!wait_or_abort(sh, &sh->scale_full[t % kScales], (t / kScales) & 1u)) return false;
+                const float2 ks = *reinterpret_cast<const float2*>(&sh->scale[t % kScales]);
+                // at least the smallest normal number: a masked score, -inf, times 0 would be NaN
+                const float c0 = ks.x * factor < kTiny ? kTiny : ks.x * factor, c1 = ks.y * factor < kTiny ? kTiny : ks.y * factor;
+                if (!softmax_tile<kDiag>(sh, x, t_s, t_o, kDiag ? lim + min(tok, live - 1) : 0, kDiag ? lim + min(tok_lo, live - 1) : 0,
+                                         kDiag ? lim + min(tok_hi, live - 1) : 0, j == 0,
+                                         (tiles - 1) & 1u, c0, c1, alive, m_run, m_used, l, turn_bar, turn_parity,
+                                         (both && (x == 0 || j < it.n_a)) ? &sh->turn[x] : nullptr))
+                    return false;
+                // the turn is handed over by A after each of its tiles, by B after those that followed one of A's
+                ++tiles;
+                return true;
+            };
+            const int n_plain = min(n_x, (first_lim + 1) / kTileKV);  // tiles j with j * 128 + 127 <= first_lim
+            int j = 0;
+            const bool dead = tok_lo >= live;  // the whole warp lies behind the sequence's last row
+            if (dead) {
+                for (; ok && j < n_x; ++j) ok = tile_step(j, std::integral_constant<int, 2>{});
+            } else {
+                for (; ok && j < n_plain; ++j) ok = tile_step(j, std::integral_constant<int, 0>{});
+                for (; ok && j < n_x; ++j) ok = tile_step(j, std::integral_constant<int, 1>{});
+            }
+            if (!ok) break;
+            // ---- epilogue: O / l -> bf16 -> global, then hand O back to the MMA thread ----
+            if (!(ok = wait_or_abort(sh, &sh->o_full[x], (tiles - 1) & 1u))) break;
+            tc_fence_after();
+            if constexpr (std::is_same<P, Split>::value) {
+                if (it.kv0 >= 0) {  // a run of a split item: its O, maximum and sum as they are
+                    float* part = p.partials + ((size_t)blockIdx.x * 2 + x) * kPartialFloats;
+                    if (!dead) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t ov[32];
+                            tmem_ld32(t_o + c * 32, ov);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                *reinterpret_cast<uint4*>(part + row * kD + c * 32 + i * 4) =
+                                    make_uint4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
+                        }
+                        part[kTileQ * kD + row] = m_used;
+                        part[kTileQ * kD + kTileQ + row] = l;
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&sh->o_empty[x]);
+                        mbar_arrive(&sh->item_empty[k % kItemRing]);
+                    }
+                    if (x == 0 && both) ok = wait_or_abort(sh, &sh->turn[1], turns_seen++ & 1u);
+                    continue;
+                }
+            }
+            const float inv = 1.0f / l;
+            const int head = it.head + x * p.pack.dh + tok_head;
+            __nv_bfloat16* orow = p.out + ((size_t)(it.seq_start + q_pos + tok) * p.H + head) * kD;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (dead) break;
+                uint32_t ov[32];
+                tmem_ld32(t_o + c * 32, ov);
+                tmem_wait_ld();
+                if (tok < live && p.wide) {  // whole sectors: half the store instructions
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            w[e] = pack_bf16(__uint_as_float(ov[16 * i + 2 * e]) * inv, __uint_as_float(ov[16 * i + 2 * e + 1]) * inv);
+                        store_32bytes(orow + c * 32 + i * 16, w);
+                    }
+                } else if (tok < live) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint4 w;
+                        w.x = pack_bf16(__uint_as_float(ov[8 * i + 0]) * inv, __uint_as_float(ov[8 * i + 1]) * inv);
+                        w.y = pack_bf16(__uint_as_float(ov[8 * i + 2]) * inv, __uint_as_float(ov[8 * i + 3]) * inv);
+                        w.z = pack_bf16(__uint_as_float(ov[8 * i + 4]) * inv, __uint_as_float(ov[8 * i + 5]) * inv);
+                        w.w = pack_bf16(__uint_as_float(ov[8 * i + 6]) * inv, __uint_as_float(ov[8 * i + 7]) * inv);
+                        *reinterpret_cast<uint4*>(orow + c * 32 + i * 8) = w;
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sh->o_empty[x]);
+                mbar_arrive(&sh->item_empty[k % kItemRing]);  // only now: the next claim waits for it
+            }
+            // B's last turn.  Else A, two hand-overs further with the next item's first tile, could lap a warp of B that was
+            // held up in front of its last wait (2.7 us would do), and the parity would alias.
+            if (x == 0 && both) ok = wait_or_abort(sh, &sh->turn[1], turns_seen++ & 1u);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
+        // ============================ converting warps =============================
+        const int w = warp - 12, r4 = lane >> 3, part = lane & 7;  // four rows of 128 bytes (16 per lane) at a time
+        uint32_t t = 0;
+        bool ok = true;
+        Item it;
+        for (uint32_t k = 0; ok && next_item(sh, k, it); ++k) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->item_empty[k % kItemRing]);
+            // ---- Q: rows of the item's tiles, those behind the sequence's end as zeros ----
+            if (k > 0 && !(ok = wait_or_abort(sh, &sh->q_empty, (k - 1) & 1u))) break;
+            for (int x = 0; x < (it.n_b > 0 ? 2 : 1); ++x) {
+                const int q_pos = it.q0 + x * p.pack.dq, live = min(p.pack.tokens, it.len - q_pos);
+#pragma unroll 1
+                for (int s = 0; s < 8; s += 4) {
+                    uint4 a[4], b[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int row = w * 32 + (s + u) * 4 + r4;
+                        const int tok = row / p.pack.heads;
+                        a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
+                        if (tok < live) {
+                            const int head = it.head + x * p.pack.dh + row - tok * p.pack.heads;
+                            const uint4* src = reinterpret_cast<const uint4*>(
+                                p.in.q + ((size_t)(it.seq_start + q_pos + tok) * p.H + head) * kD + part * 16);
+                            a[u] = __ldg(src), b[u] = __ldg(src + 1);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int row = w * 32 + (s + u) * 4 + r4;
+                        const uint32_t in[8] = {a[u].x, a[u].y, a[u].z, a[u].w, b[u].x, b[u].y, b[u].z, b[u].w};
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = max(top, max(in[e] & 0x7fffu, in[e] >> 16 & 0x7fffu));
+#pragma unroll
+                        for (int step = 1; step < 8; step <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
+                        // divided by 2^(e - up): 1.m * 2^(e - 127) becomes 224 < .. <= 448
+                        const uint32_t up = (top & 0x7fu) <= 0x60u ? 8 : 7, e = min(max(top == 0 ? 127u + up : top >> 7, 9u), 254u);
+                        const float down = __uint_as_float((254u + up - e) << 23);
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float f[4], g[4];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                f[2 * h] = __uint_as_float(in[2 * c + h] << 16) * down;
+                                f[2 * h + 1] = __uint_as_float(in[2 * c + h] & 0xffff0000u) * down;
+                            }
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) f[h] = fabsf(f[h]) < INFINITY ? f[h] : __uint_as_float(0x7fffffffu);
+                            const uint32_t h0 = q8::to_e4m3x2(f[0], f[1]), h1 = q8::to_e4m3x2(f[2], f[3]);
+                            const float2 g0 = q8::e4m3x2_to_float2(h0), g1 = q8::e4m3x2_to_float2(h1);
+                            g[0] = f[0] - g0.x, g[1] = f[1] - g0.y, g[2] = f[2] - g1.x, g[3] = f[3] - g1.y;
+                            hi[c] = h0 | h1 << 16;
+                            lo[c] = q8::to_e4m3x2(g[0], g[1]) | q8::to_e4m3x2(g[2], g[3]) << 16;
+                        }
+                        uint8_t* to = smem + x * kTileBytes + row * 128 + ((part ^ (row & 7)) << 4);
+                        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4*>(to + kByteTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        if (part == 0) sh->q_factor[k & 1][x][row] = __uint_as_float((e - up) << 23);
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sh->factor_full[k & 1]);
+                mbar_arrive(&sh->q_full);
+            }
+            // ---- V, tile by tile ----
+            for (int j = 0; j < it.n_kv; ++j, ++t) {
+                const int slot = t % kSlots, vs = t % kVSlots, own = it.len_k - j * kTileKV;
+                if (!(ok = wait_or_abort(sh, &sh->scale_full[t % kScales], (t / kScales) & 1u))) break;
+                const float scale = w < 2 ? sh->scale[t % kScales].z : sh->scale[t % kScales].w;
+                if (!(ok = wait_or_abort(sh, &sh->vb_full[slot], (t / kSlots) & 1u))) break;
+                const uint8_t* from = smem + kVBytes + slot * kByteTile + (w * 32 + r4) * 128;
+                uint4 in[8];
+#pragma unroll
+                for (int s = 0; s < 8; ++s) in[s] = *reinterpret_cast<const uint4*>(from + s * 512 + ((part ^ ((s * 4 + r4) & 7)) << 4));
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->vb_empty[slot]);
+                if (!(ok = wait_or_abort(sh, &sh->v_empty[vs], ((t / kVSlots) & 1u) ^ 1u))) break;
+                uint8_t* to = smem + kV + vs * kTileBytes + (part >> 2) * kPanelBytes + (w * 32 + r4) * 128;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {
+                    const uint32_t b[4] = {in[s].x, in[s].y, in[s].z, in[s].w};
+                    uint32_t o[8];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const float2 f = q8::e4m3x2_to_float2(b[c] & 0xffffu), g = q8::e4m3x2_to_float2(b[c] >> 16);
+                        o[2 * c] = pack_bf16(f.x * scale, f.y * scale);
+                        o[2 * c + 1] = pack_bf16(g.x * scale, g.y * scale);
+                    }
+                    if (w * 32 + s * 4 + r4 >= own) {  // behind the sequence's end: 0 * garbage would poison the row
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) o[c] = 0u;
+                    }
+                    // Dims 16 part .. + 15 are chunks 2 (part % 4) and + 1 of a panel's row.  Lanes of the second panel take
+                    // theirs in the other order, so that eight lanes always write eight different banks' chunks.
+                    const int r7 = (s * 4 + r4) & 7, first = 2 * (part & 3) + (part >> 2), second = first ^ 1;
+                    const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+                    *reinterpret_cast<uint4*>(to + s * 512 + ((first ^ r7) << 4)) = part < 4 ? lo : hi;
+                    *reinterpret_cast<uint4*>(to + s * 512 + ((second ^ r7) << 4)) = part < 4 ? hi : lo;
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh->v_full[vs]);
+            }
+        }
+    }
+
+    // ---- teardown: everyone meets here, then the allocating warp frees tensor memory ----
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1 && tmem != 0xFFFFFFFFu) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+static int ensure_attr() {
+    static std::mutex mu;
+    static bool done[64];
+    int dev = 0;
+    NVLLM_CUDA_OK(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev >= 0 && dev < 64 && !done[dev]) {
+        for (const void* f : {(const void*)paged_prefill_q8_kernel<Whole>, (const void*)paged_prefill_q8_kernel<Split>}) {
+            cudaFuncAttributes a;
+            NVLLM_CUDA_OK(cudaFuncGetAttributes(&a, f));
+            if (a.numRegs != 128) return fail(NVLLM_B200_ECUDA, "paged_prefill_q8: built with %d registers, not the 128 it shares out", a.numRegs);
+            NVLLM_CUDA_OK(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+        }
+        done[dev] = true;
+    }
+    return NVLLM_B200_OK;
+}
+
+static int make_byte_map(CUtensorMap* map, const void* base, int heads, int64_t tokens) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return fail(NVLLM_B200_EDRIVER, "cuTensorMapEncodeTiled entry point not available");
+    cuuint64_t dims[3] = {(cuuint64_t)kD, (cuuint64_t)heads, (cuuint64_t)tokens};
+    cuuint64_t strides[2] = {(cuuint64_t)kD, (cuuint64_t)heads * kD};
+    cuuint32_t box[3] = {kD, 1, kTileKV};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(NVLLM_B200_EDRIVER, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+    return NVLLM_B200_OK;
+}
+
+}  // namespace prefill_q8
+
+namespace prefill {
+int launch_bytes(const Params& p, const SplitParams* split, const Bytes& in, const void* q, const void* k, const void* v, int64_t slots,
+                 int KVH, cudaLaunchConfig_t cfg) {
+    using namespace prefill_q8;
+    int rc = ensure_attr();
+    if (rc) return rc;
+    CUtensorMap tm_k, tm_v;
+    if ((rc = make_byte_map(&tm_k, k, KVH, slots))) return rc;
+    if ((rc = make_byte_map(&tm_v, v, KVH, slots))) return rc;
+    const Source src = {(const __nv_bfloat16*)q, in.k_scale, in.v_scale, in.NB, KVH};
+    cfg.blockDim = dim3(prefill_q8::kThreads);
+    cfg.dynamicSmemBytes = prefill_q8::kSmemBytes;
+    if (split) {
+        Split s;
+        static_cast<SplitParams&>(s) = *split;
+        s.in = src;
+        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_prefill_q8_kernel<Split>, tm_k, tm_v, s));
+    } else {
+        Whole s;
+        static_cast<Params&>(s) = p;
+        s.in = src;
+        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_prefill_q8_kernel<Whole>, tm_k, tm_v, s));
+    }
+    return NVLLM_B200_OK;
+}
+}  // namespace prefill
+
+int read_prefill_q8_flags(int* out) {
+    NVLLM_CUDA_OK(cudaMemcpyFromSymbol(out, prefill_q8::g_error_flag, sizeof(int)));
+    return NVLLM_B200_OK;
+}
+int clear_prefill_q8_flags() {
+    const int zero = 0;
+    NVLLM_CUDA_OK(cudaMemcpyToSymbol(prefill_q8::g_error_flag, &zero, sizeof(int)));
+    return NVLLM_B200_OK;
+}
+}  // namespace nvllm

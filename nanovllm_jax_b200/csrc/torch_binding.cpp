@@ -39,6 +39,7 @@ struct Api {
     decltype(&nvllm_b200_paged_decode_q8_workspace_bytes) decode_q8_workspace_bytes;
     decltype(&nvllm_b200_paged_decode_q8) paged_decode_q8;
     decltype(&nvllm_b200_decode_step_q8) decode_step_q8;
+    decltype(&nvllm_b200_paged_prefill_q8) paged_prefill_q8;
     decltype(&nvllm_b200_copy_pages) copy_pages;
 } api = {};
 PyObject* check_fn = nullptr;  // raises NvllmError for a non-zero status, from the library's thread-local text
@@ -709,6 +710,37 @@ PyObject* decode_step_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// paged_prefill_q8(q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, scale, block_size,
+//                  out, cu_seqlens_host)
+PyObject* paged_prefill_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return entry("paged_prefill_q8", n, 13, [&]() -> PyObject* {
+        const at::Tensor& q = need(a[0], "q", at::kBFloat16, 3);
+        const Cache8 c = cache8(a + 1);
+        const at::Tensor& bt = need(a[5], "block_tables", at::kInt, 2);
+        const at::Tensor& cu = need(a[6], "cu_seqlens_q", at::kInt, 1);
+        const at::Tensor& cu_k = need(a[7], "cu_seqlens_k", at::kInt, 1);
+        const int max_seqlen_q = to_bound(a[8]);
+        const float scale = to_float(a[9]);
+        fits_q(c, q, to_int(a[10]));
+        same_device(q, {&c.k, &c.v, &c.k_scale, &c.v_scale, &bt, &cu, &cu_k});
+        const int64_t t = q.size(0);
+        const int h = (int)q.size(1), b = (int)cu.size(0) - 1;
+        if (b < 0 || cu_k.size(0) != b + 1 || bt.size(0) != b) raise(PyExc_ValueError, "cu_seqlens_k / block_tables batch mismatch");
+        const HostLengths host(a[12], b + 1);
+        const Site site(q);
+        const at::Tensor out = output_like(a[11], q);
+        same_device(q, {&out});
+        zero_uncovered(host, b, out, t);
+        const at::Tensor ws = site.scratch(std::max<size_t>(api.prefill_workspace_bytes(t, b, h, c.kvh, c.d), 256));
+        call([&] {
+            return api.paged_prefill_q8(ptr(q), ptr(c.k), ptr(c.v), fptr(c.k_scale), fptr(c.v_scale), iptr(cu), iptr(cu_k), iptr(bt),
+                                        host.data, mptr(out), mptr(ws), ws.nbytes(), t, b, max_seqlen_q, h, c.kvh, c.d, c.nb, c.block,
+                                        (int)bt.size(1), scale, site.stream);
+        });
+        return result(a[11], out);
+    });
+}
+
 // copy_pages(caches, src, dst, block_size, tokens, block_tables)
 PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     return entry("copy_pages", n_args, 6, [&]() -> PyObject* {
@@ -839,6 +871,7 @@ PyObject* bind(PyObject*, PyObject* args) {
         {"nvllm_b200_paged_decode_q8_workspace_bytes", (void**)&api.decode_q8_workspace_bytes},
         {"nvllm_b200_paged_decode_q8", (void**)&api.paged_decode_q8},
         {"nvllm_b200_decode_step_q8", (void**)&api.decode_step_q8},
+        {"nvllm_b200_paged_prefill_q8", (void**)&api.paged_prefill_q8},
         {"nvllm_b200_copy_pages", (void**)&api.copy_pages},
     };
     for (const auto& e : entries) {
@@ -866,6 +899,7 @@ PyMethodDef methods[] = {
     FAST("store_kvcache_q8", store_kvcache_q8),
     FAST("paged_decode_q8", paged_decode_q8),
     FAST("decode_step_q8", decode_step_q8),
+    FAST("paged_prefill_q8", paged_prefill_q8),
     FAST("copy_pages", copy_pages),
     FAST("workspace", py_workspace),
     FAST("fill_decode_metadata", fill_decode_metadata),

@@ -952,11 +952,12 @@ static int64_t item_capacity(int64_t T, int B, int span) { return T / span + B +
 static size_t list_bytes(int64_t T, int B, int span) { return ((size_t)(2 * item_capacity(T, B, span) + 1) * 16 + 255) & ~size_t(255); }
 
 // Common launcher.  kv_tokens: extent of the token axis of k / v (T for packed tensors, the slot count of the cache).
-// sc (may be null): the step's K/V scatter.
+// sc (may be null): the step's K/V scatter.  bytes (may be null): the pages are in 8 bits, with these scales.
 static int launch(const char* who, const void* q, const void* k, const void* v, int64_t kv_tokens,
                   const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* block_tables, int MB,
                   int block_size, const int32_t* cu_seqlens_host, void* out, void* workspace, size_t workspace_bytes,
-                  int64_t T, int B, int max_seqlen, int H, int KVH, int D, float scale, const Scatter* sc, void* stream) {
+                  int64_t T, int B, int max_seqlen, int H, int KVH, int D, float scale, const Scatter* sc, void* stream,
+                  const Bytes* bytes = nullptr) {
     if (T < 0 || B < 0 || H <= 0 || KVH <= 0)
         return fail(NVLLM_B200_EINVAL, "%s: bad size (T=%lld B=%d H=%d KVH=%d)", who, (long long)T, B, H, KVH);
     if (D != kD) return fail(NVLLM_B200_EUNSUPPORTED, "%s: head_dim %d (only 128)", who, D);
@@ -1038,9 +1039,11 @@ static int launch(const char* who, const void* q, const void* k, const void* v, 
     int rc = ensure_attr();
     if (rc) return rc;
     CUtensorMap tm_q, tm_k, tm_v;
-    if ((rc = make_map(&tm_q, q, H, T, pack.heads, pack.tokens))) return rc;
-    if ((rc = make_map(&tm_k, k, KVH, kv_tokens))) return rc;
-    if ((rc = make_map(&tm_v, v, KVH, kv_tokens))) return rc;
+    if (!bytes) {
+        if ((rc = make_map(&tm_q, q, H, T, pack.heads, pack.tokens))) return rc;
+        if ((rc = make_map(&tm_k, k, KVH, kv_tokens))) return rc;
+        if ((rc = make_map(&tm_v, v, KVH, kv_tokens))) return rc;
+    }
 
     p.items = (const int4*)workspace;
     p.cu_seqlens = cu_seqlens_q;
@@ -1096,12 +1099,18 @@ static int launch(const char* who, const void* q, const void* k, const void* v, 
         sp.splits = splits;
         sp.ctas = (int)(pairs * p.per_pair * splits);
         cfg.gridDim = dim3((unsigned)sp.ctas);
-        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<SplitParams>, tm_q, tm_k, tm_v, sp));
+        if (bytes) {
+            if ((rc = launch_bytes(p, &sp, *bytes, q, k, v, kv_tokens, KVH, cfg))) return rc;
+        } else {
+            NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<SplitParams>, tm_q, tm_k, tm_v, sp));
+        }
         cfg.gridDim = dim3((unsigned)(pairs * p.per_pair), 2, kTileQ / 8);
         cfg.blockDim = dim3(kCombineThreads);
         cfg.dynamicSmemBytes = 0;
         NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, prefill_combine_kernel, sp));
-    } else if (brief)
+    } else if (bytes)
+        return launch_bytes(p, nullptr, *bytes, q, k, v, kv_tokens, KVH, cfg);
+    else if (brief)
         NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<ShortParams>, tm_q, tm_k, tm_v, p));
     else
         NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<Params>, tm_q, tm_k, tm_v, (const Params&)p));
@@ -1160,6 +1169,24 @@ extern "C" int nvllm_b200_paged_prefill(const void* q, const void* k_cache, cons
     return prefill::launch("paged_prefill", q, k_cache, v_cache, (int64_t)NB * block_size, cu_seqlens_q, cu_seqlens_k,
                            block_tables, MB, block_size, cu_seqlens_q_host, out, workspace, workspace_bytes, T, B,
                            max_seqlen_q, H, KVH, D, scale, nullptr, stream);
+}
+
+extern "C" int nvllm_b200_paged_prefill_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                                           const float* v_scale, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                           const int32_t* block_tables, const int32_t* cu_seqlens_q_host, void* out,
+                                           void* workspace, size_t workspace_bytes, int64_t T, int B, int max_seqlen_q, int H,
+                                           int KVH, int D, int NB, int block_size, int MB, float scale, void* stream) {
+    using namespace nvllm;
+    const char* who = "paged_prefill_q8";
+    if (!block_tables || MB <= 0) return fail(NVLLM_B200_EINVAL, "%s: block_tables required", who);
+    if (!k_scale || !v_scale) return fail(NVLLM_B200_EINVAL, "%s: null pointer", who);
+    if (((uintptr_t)k_scale | (uintptr_t)v_scale) & 3) return fail(NVLLM_B200_EINVAL, "%s: scales must be 4-byte aligned", who);
+    int rc = prefill::check_pages(who, NB, block_size);
+    if (rc) return rc;
+    const prefill::Bytes bytes = {k_scale, v_scale, NB};
+    return prefill::launch(who, q, k_cache, v_cache, (int64_t)NB * block_size, cu_seqlens_q, cu_seqlens_k, block_tables, MB, block_size,
+                           cu_seqlens_q_host, out, workspace, workspace_bytes, T, B, max_seqlen_q, H, KVH, D, scale, nullptr, stream,
+                           &bytes);
 }
 
 extern "C" int nvllm_b200_prefill_step(const void* q, const void* k, const void* v, void* k_cache, void* v_cache,

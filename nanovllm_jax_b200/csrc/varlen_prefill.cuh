@@ -341,5 +341,13 @@ inline bool lone_tiles(int64_t max_tiles, int splits, int lone_splits, int64_t l
 }
 inline size_t partials_bytes(int sms) { return (size_t)sms * 2 * kPartialFloats * 4; }
 
+// Keys and values in 8-bit pages: the main kernel is another one (paged_prefill_q8.cu).  `split`: for runs, or null.
+struct Bytes {
+    const float *k_scale, *v_scale;
+    int NB;
+};
+int launch_bytes(const Params& p, const SplitParams* split, const Bytes& in, const void* q, const void* k, const void* v, int64_t slots,
+                 int KVH, cudaLaunchConfig_t cfg);
+
 }  // namespace prefill
 }  // namespace nvllm

@@ -7,6 +7,7 @@ Mirrors, name for name, what the model and the model runner of nanovllm_jax touc
     paged_attention, paged_prefill_attention, PALLAS_AVAILABLE,
     Attention(num_heads, head_dim, scale, num_kv_heads, block_size=256)
         .set_kv_cache(k_cache, v_cache)     # [num_blocks, block_size, num_kv_heads, head_dim] bf16
+        .set_kv_cache_q8(k_cache, v_cache, k_scale, v_scale)    # or: the same in 8 bits, with scales (no counterpart there)
         .__call__(q, k, v, context) -> o    # same shape and dtype as q
 
 Arrays are torch CUDA tensors.  Head counts are per rank, as in the reference
@@ -81,11 +82,31 @@ class Attention:
         self.block_size = block_size
         self.k_cache = None
         self.v_cache = None
+        self.k_scale = None  # set where the cache is in 8 bits
+        self.v_scale = None
 
     def set_kv_cache(self, k_cache, v_cache):
         """Called by the model runner after it allocates the cache (reference :326-329)."""
         self.k_cache = k_cache
         self.v_cache = v_cache
+        self.k_scale = self.v_scale = None
+
+    def set_kv_cache_q8(self, k_cache, v_cache, k_scale, v_scale):
+        """A cache in 8 bits instead: float8_e4m3fn [num_blocks, block_size, num_kv_heads, head_dim] and fp32 scales
+        [num_blocks, block_size / 64, num_kv_heads] (see ``ops.store_kvcache_q8``).  Prompts without a cached prefix attend to
+        the k and v that they bring, in bf16; decode steps and prompts behind a cached prefix to what the cache holds."""
+        self.k_cache = k_cache
+        self.v_cache = v_cache
+        self.k_scale = k_scale
+        self.v_scale = v_scale
+
+    def _call_q8(self, q, k, v, context: AttentionContext):
+        cache = (self.k_cache, self.v_cache, self.k_scale, self.v_scale)
+        if not context.is_prefill:
+            return _lib.binding().decode_step_q8(q, k, v, *cache, context.slot_mapping, context.block_tables,
+                                                 context.context_lens, self.scale, self.block_size, None, True)
+        ops.store_kvcache_q8(k.contiguous(), v.contiguous(), *cache, context.slot_mapping)
+        return self._prefill_attention(q, k, v, context)
 
     def _prefill_attention(self, q, k, v, context: AttentionContext):
         batch_size = context.cu_seqlens_q.shape[0] - 1
@@ -96,6 +117,11 @@ class Attention:
             # rows were stored by __call__ just before).
             if self.k_cache is None or self.v_cache is None:
                 raise RuntimeError("prefill over a cached prefix needs the KV cache: call set_kv_cache first")
+            if self.k_scale is not None:
+                return ops.paged_prefill_q8(q.to(torch.bfloat16).contiguous(), self.k_cache, self.v_cache, self.k_scale,
+                                            self.v_scale, context.block_tables, context.cu_seqlens_q,
+                                            context.cu_seqlens_k, context.max_seqlen_q, self.scale, self.block_size,
+                                            cu_seqlens_host=getattr(context, "cu_seqlens_host", None))
             return ops.paged_prefill(q.to(self.k_cache.dtype).contiguous(), self.k_cache, self.v_cache,
                                      context.block_tables, context.cu_seqlens_q, context.cu_seqlens_k,
                                      context.max_seqlen_q, self.scale, self.block_size,
@@ -112,12 +138,18 @@ class Attention:
     def _decode_attention(self, q, context: AttentionContext):
         if self.k_cache is None or self.v_cache is None:
             raise RuntimeError("decode attention needs the KV cache: call set_kv_cache first")
+        if self.k_scale is not None:
+            return ops.paged_decode_q8(q.to(torch.bfloat16).contiguous(), self.k_cache, self.v_cache, self.k_scale,
+                                       self.v_scale, context.block_tables, context.context_lens, self.scale,
+                                       self.block_size)
         q = q.to(self.k_cache.dtype)  # reference :386-387
         return paged_attention(q=q, k_cache=self.k_cache, v_cache=self.v_cache, block_tables=context.block_tables,
                                context_lens=context.context_lens, scale=self.scale, block_size=self.block_size)
 
     def __call__(self, q, k, v, context: AttentionContext):
         """q [T, H, D]; k, v [T, KVH, D]; returns [T, H, D].  Stores k/v first, then attends (reference :436-480)."""
+        if self.k_scale is not None:
+            return self._call_q8(q, k, v, context)
         if not context.is_prefill and self.k_cache is not None and self.v_cache is not None:
             # decode: the scatter of the step's K/V rows and the attention over the pages go down as one C call
             # (same result as the two calls of the reference, :465-467 then :476-478)

@@ -136,6 +136,16 @@ def decode_step_q8(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_ca
                                          context_lens, scale, block_size, out, False)
 
 
+def paged_prefill_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                     cu_seqlens_k: torch.Tensor, max_seqlen_q: int, scale: float, block_size: int,
+                     out: torch.Tensor | None = None, cu_seqlens_host=None) -> torch.Tensor:
+    """``paged_prefill`` over an 8-bit paged cache (see ``store_kvcache_q8``; block_size a multiple of 128): causal attention of
+    packed new tokens over their whole sequences.  The new tokens' rows must already be in the cache."""
+    return _lib.binding().paged_prefill_q8(q, k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_q, cu_seqlens_k,
+                                           max_seqlen_q, scale, block_size, out, _host_lengths(cu_seqlens_host))
+
+
 def copy_pages(caches, src: torch.Tensor, dst: torch.Tensor, block_size: int, tokens: torch.Tensor | None = None,
                block_tables: torch.Tensor | None = None) -> None:
     """In place: ``cache[dst[i]] = cache[src[i]]`` for every pair i and every tensor of ``caches``, in one launch.

@@ -120,3 +120,15 @@ def test_shapes_types_and_strides():
                        (dict(block=0), ValueError)):
         with pytest.raises(error):
             copy(**bad)
+
+
+def test_prefill(lib):
+    from nanovllm_jax_b200 import _lib
+
+    def prefill(q=P, cache=P, scale=P, tables=P, ws=P, wsn=1 << 30, t=5, b=1, m=5, h=8, kvh=2, d=128, nb=4, block=128, mb=2, s=0.1):
+        return lib.nvllm_b200_paged_prefill_q8(q, cache, P, scale, P, P, P, tables, None, P, ws, wsn, t, b, m, h, kvh, d, nb, block, mb, s, None)
+    assert prefill(d=64) == prefill(block=64) == prefill(block=192) == prefill(h=7) == prefill(b=70000) == _lib.EUNSUPPORTED
+    assert prefill(t=-1) == prefill(nb=0) == prefill(mb=0) == prefill(s=0.0) == prefill(m=0) == _lib.EINVAL
+    assert prefill(q=None) == prefill(scale=None) == prefill(scale=P + 2) == prefill(tables=None) == prefill(cache=P + 8) == _lib.EINVAL
+    assert prefill(ws=None) == prefill(wsn=16) == _lib.EWORKSPACE
+    assert prefill(t=0, q=None) == prefill(b=0, q=None) == _lib.OK
