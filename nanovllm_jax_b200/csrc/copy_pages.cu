@@ -5,8 +5,9 @@
 // a launch per tensor would cost a 36-layer model 144 of them.
 //
 // Pure data movement: 2 bytes of traffic per byte copied.  A page of a tensor is cut into pieces of kPieceBytes; a CTA takes
-// one piece, or a few where there are many.  A CTA looks through the pairs for one that forbids its own (see refused) while
-// its loads are in flight.
+// one piece of one tensor (blockIdx.y: its entry of the parameters is then read by all threads at once; found by a search
+// among the pieces of all tensors, four pages of 144 tensors took 30 us instead of 13), or a few where there are many.  A CTA
+// looks through the pairs for one that forbids its own while its loads are in flight.
 #include "common.cuh"
 
 #include <algorithm>
@@ -17,45 +18,47 @@ namespace pages {
 constexpr int kThreads = 256;
 constexpr int kUnroll = 8;
 constexpr int kPieceBytes = kThreads * kUnroll * 16;  // 32 KB
-constexpr int kMaxCaches = 128;                       // per launch: 2 KB of parameters
+constexpr int kFew = 16, kMany = 512;                 // tensors of a launch: the parameters are of one of two sizes
 
 __device__ int g_error_flag = 0;  // bit 7 (128): a pair was not carried out
 
 struct Cache {
     uint8_t* base;
-    int row_bytes;
-    int first_piece;  // of this cache among a pair's
+    int rows, row_bytes;  // of a page; bytes of a row
 };
-struct Params {
-    Cache caches[kMaxCaches];
-    int rows[kMaxCaches];  // of a page
-    int num_caches, pieces;  // pieces of a pair, over all caches
+struct Common {
     const int32_t *src, *dst, *tokens;
     int n, block_size;
     int64_t NB;
-    int64_t copy_ctas;  // CTAs behind them take the tables
-    int64_t units;      // n * pieces
+    int pieces;        // of the largest page
+    int copy_ctas;     // per tensor; CTAs behind them take the tables
+    int64_t units;     // n * pieces
     int32_t* tables;
     int64_t table_entries;
 };
+template <int kCaches>
+struct Params : Common {
+    Cache caches[kCaches];
+};
 
-__device__ __forceinline__ bool in_pool(const Params& p, int page) { return page >= 0 && page < p.NB; }
+__device__ __forceinline__ bool in_pool(const Common& p, int page) { return page >= 0 && page < p.NB; }
 
 // Whether pair j stands in the way of another pair, (s, d) at place i: it reads the page that i would write, or writes the same
 // page later in the list.  With these left out no page is both read and written, and none is written twice.
-__device__ __forceinline__ bool forbids(const Params& p, int j, int i, int d) {
+__device__ __forceinline__ bool forbids(const Common& p, int j, int i, int d) {
     if (j == i) return false;
     const int sj = __ldg(p.src + j), dj = __ldg(p.dst + j);
     return in_pool(p, sj) && in_pool(p, dj) && (sj == d || (dj == d && j > i));
 }
 
-__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ Params p) {
-    const int tid = threadIdx.x, lane = tid & 31;
+template <int kCaches>
+__global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ Params<kCaches> p) {
+    const int tid = threadIdx.x;
     griddep_wait();
     griddep_launch_dependents();
-    if ((int64_t)blockIdx.x >= p.copy_ctas) {  // the tables: an entry that names a source names its destination now
-        const int64_t at = ((int64_t)blockIdx.x - p.copy_ctas) * kThreads + tid;
-        if (at >= p.table_entries) return;
+    if ((int)blockIdx.x >= p.copy_ctas) {  // the tables: an entry that names a source names its destination now
+        const int64_t at = (int64_t)(blockIdx.x - p.copy_ctas) * kThreads + tid;
+        if (blockIdx.y > 0 || at >= p.table_entries) return;
         const int page = p.tables[at];
         if (!in_pool(p, page)) return;
         for (int i = 0; i < p.n; ++i) {
@@ -70,28 +73,24 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_const
         }
         return;
     }
+    const Cache cache = p.caches[blockIdx.y];
+    const int64_t page_bytes = (int64_t)cache.rows * cache.row_bytes;
+    const bool wide = (((uintptr_t)cache.base | (uintptr_t)cache.row_bytes) & 15) == 0;
     for (int64_t u = blockIdx.x; u < p.units; u += p.copy_ctas) {
-        const int i = (int)(u / p.pieces), piece = (int)(u - (int64_t)i * p.pieces);
+        const int i = (int)(u / p.pieces);
+        const int64_t off = (u - (int64_t)i * p.pieces) * kPieceBytes;
+        if (off >= page_bytes) continue;
         const int s = __ldg(p.src + i), d = __ldg(p.dst + i);
         if (!in_pool(p, s) || !in_pool(p, d) || s == d) continue;
-        int c = -1;  // the last cache that begins at or before the piece
-#pragma unroll
-        for (int w = 0; w < kMaxCaches; w += 32)
-            c += __popc(__ballot_sync(0xffffffffu, w + lane < p.num_caches && p.caches[w + lane].first_piece <= piece));
-        const Cache cache = p.caches[c];
-        const int rows = p.rows[c];
-        const int64_t page_bytes = (int64_t)rows * cache.row_bytes;
         int64_t live = page_bytes;
         if (p.tokens != nullptr) {
             const int64_t t = max(0, min(__ldg(p.tokens + i), p.block_size));
-            live = (t * rows + p.block_size - 1) / p.block_size * cache.row_bytes;
+            live = (t * cache.rows + p.block_size - 1) / p.block_size * cache.row_bytes;
         }
-        const int64_t off = (int64_t)(piece - cache.first_piece) * kPieceBytes;
         const int bytes = (int)min((int64_t)kPieceBytes, live - off);
-        if (bytes <= 0 && off > 0) continue;  // the cache's first piece looks at the pair even where nothing is live
+        if (bytes <= 0 && off > 0) continue;  // a page's first piece looks at the pair even where nothing is live
         const uint8_t* const from = cache.base + s * page_bytes + off;
         uint8_t* const to = cache.base + d * page_bytes + off;
-        const bool wide = (((uintptr_t)cache.base | (uintptr_t)cache.row_bytes) & 15) == 0;
         uint4 x[kUnroll];
         if (wide) {
 #pragma unroll
@@ -165,21 +164,15 @@ extern "C" int nvllm_b200_copy_pages(void* const* caches_host, const int32_t* pa
     cfg.stream = reinterpret_cast<cudaStream_t>(stream);
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 1 : 0;
-    int c0 = 0;
-    do {
-        Params p = {};
-        int64_t pieces = 0;
-        for (; c0 < num_caches && p.num_caches < kMaxCaches; ++c0) {
-            const int64_t page = (int64_t)page_rows_host[c0] * row_bytes_host[c0];
-            const int64_t mine = (page + kPieceBytes - 1) / kPieceBytes;
-            if (pieces + mine > 0x3fffffffLL) {
-                if (p.num_caches == 0) return fail(NVLLM_B200_EUNSUPPORTED, "%s: page of %lld bytes too large", who, (long long)page);
-                break;
-            }
-            p.caches[p.num_caches] = Cache{(uint8_t*)caches_host[c0], (int)row_bytes_host[c0], (int)pieces};
-            p.rows[p.num_caches++] = page_rows_host[c0];
-            pieces += mine;
+    for (int c0 = 0; c0 < num_caches || c0 == 0; c0 += kMany) {
+        const int count = std::min(num_caches - c0, kMany);
+        Params<kMany> p = {};
+        int64_t pieces = 1;
+        for (int c = 0; c < count; ++c) {
+            p.caches[c] = Cache{(uint8_t*)caches_host[c0 + c], page_rows_host[c0 + c], (int)row_bytes_host[c0 + c]};
+            pieces = std::max(pieces, ((int64_t)page_rows_host[c0 + c] * row_bytes_host[c0 + c] + kPieceBytes - 1) / kPieceBytes);
         }
+        if (pieces > 0x3fffffffLL) return fail(NVLLM_B200_EUNSUPPORTED, "%s: pages too large", who);
         p.pieces = (int)pieces;
         p.src = src;
         p.dst = dst;
@@ -187,17 +180,27 @@ extern "C" int nvllm_b200_copy_pages(void* const* caches_host, const int32_t* pa
         p.n = n;
         p.block_size = block_size;
         p.NB = NB;
-        p.units = (int64_t)n * pieces;
+        p.units = count > 0 ? (int64_t)n * pieces : 0;
         // A piece per CTA; with very many, up to 16 of them, so that the look through a long list of pairs is shared.
         const int64_t wave = (int64_t)sm_count() * 64;
-        const int64_t each = std::max<int64_t>(1, std::min<int64_t>(16, p.units / wave));
-        p.copy_ctas = (p.units + each - 1) / each;
-        if (c0 == num_caches) p.tables = block_tables, p.table_entries = table_entries;
-        const int64_t ctas = p.copy_ctas + (p.table_entries + kThreads - 1) / kThreads;
+        const int64_t each = std::max<int64_t>(1, std::min<int64_t>(16, p.units * count / wave));
+        const int64_t copy_ctas = (p.units + each - 1) / each;
+        const bool last = c0 + kMany >= num_caches;
+        p.tables = last ? block_tables : nullptr;
+        p.table_entries = last ? table_entries : 0;
+        const int64_t ctas = copy_ctas + (p.table_entries + kThreads - 1) / kThreads;
         if (ctas > 0x7fffffffLL) return fail(NVLLM_B200_EUNSUPPORTED, "%s: too many pages", who);
         if (ctas == 0) break;
-        cfg.gridDim = dim3((unsigned)ctas);
-        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, copy_pages_kernel, p));
-    } while (c0 < num_caches);
+        p.copy_ctas = (int)copy_ctas;
+        cfg.gridDim = dim3((unsigned)ctas, (unsigned)std::max(count, 1));
+        if (count > kFew) {
+            NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, copy_pages_kernel<kMany>, p));
+        } else {
+            Params<kFew> few;
+            static_cast<Common&>(few) = p;
+            std::copy(p.caches, p.caches + kFew, few.caches);
+            NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, copy_pages_kernel<kFew>, few));
+        }
+    }
     return NVLLM_B200_OK;
 }

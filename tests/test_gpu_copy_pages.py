@@ -44,7 +44,7 @@ def check(c, src, dst, block, tokens=None, tables=None):
 
 
 @pytest.mark.parametrize("held", ("bf16", "8 bits"))
-@pytest.mark.parametrize("kvh, block, nb, n, layers", [(1, 64, 2, 1, 1), (8, 256, 9, 4, 3), (3, 128, 40, 18, 2), (2, 512, 6, 2, 40), (1, 64, 700, 300, 1)])
+@pytest.mark.parametrize("kvh, block, nb, n, layers", [(1, 64, 2, 1, 1), (8, 256, 9, 4, 3), (3, 128, 40, 18, 2), (2, 512, 6, 2, 40), (1, 64, 700, 300, 1), (1, 64, 3, 1, 300)])
 def test_fork_and_move(held, kvh, block, nb, n, layers):
     rng = np.random.default_rng(n)
     c = caches(rng, nb, block, kvh, held, layers)
