@@ -35,15 +35,20 @@ namespace decode_q8 {
 
 using namespace decode;
 
-constexpr int kStages = 5;
-constexpr int kItemCost = 4;                          // cost of a sequence boundary in tile units
+// CTAs per SM and their stages.  Under the power limit the SM clock falls and with it what the consumer warps, bound by the latency
+// of their own chains, get done: three CTAs with three stages each hold as many bytes in flight as two with five, and give every
+// scheduler a third warp (64 sequences of 512..8192 tokens, 32 / 8 heads, at 1.69 GHz: 103 us with two, 97 with three; 256 of
+// 16..16384, 64 / 8: 229 and 214; four with two stages do not fit the registers: 144 and 307).
+constexpr int kCtas = 3;
+constexpr int kStages = 3;
+constexpr int kItemCost = 3;                          // cost of a sequence boundary in tile units
 constexpr int kMinUnits = 6;                          // units per CTA from which on more CTAs pay
 constexpr int kTileBytes = kTile * kD;                // one K or V tile, 128B-swizzled
 constexpr int kQBytes = kMaxG * kD * 2;
 constexpr int kStageBytes = 2 * kTileBytes + kQBytes;
 constexpr int kMiscBytes = 1024 + kThreads * 8;
 constexpr int kSmemBytes = kStages * kStageBytes + kOsBytes + kMiscBytes;
-static_assert(kSmemBytes + 1024 <= 228 * 1024 / 2, "two CTAs per SM");
+static_assert(kSmemBytes + 1024 <= 228 * 1024 / kCtas, "CTAs per SM");
 static_assert(kTile == q8::kGrain, "a tile has one scale");
 constexpr float kBias = 10.f;                         // log2 units: the largest probability is stored as 2^kBias ...
 constexpr float kStale = 4.f;                         // ... or up to 2^(kBias + kStale) until the maximum moves (fp16: 2^16)
@@ -83,7 +88,7 @@ __device__ __forceinline__ void arrive_behind_scales(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-__global__ void __launch_bounds__(kThreads, kCtasPerSm + 1)
+__global__ void __launch_bounds__(kThreads, kCtas)
 paged_decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Params8 p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     // swizzled tiles first: their addresses are multiples of 8 KB; the q rows of all stages behind them
@@ -530,6 +535,8 @@ decode_q8_prepare_kernel(unsigned int* __restrict__ tickets, int num_tickets, in
     }
 }
 
+static int grid() { return kCtas * sm_count(); }
+
 static int ensure_smem_attr() {
     static std::mutex mu;
     static bool done[64];
@@ -544,7 +551,7 @@ static int ensure_smem_attr() {
 }
 
 static size_t workspace_bytes_for(int B, int H, int KVH, bool step) {
-    return ticket_bytes(B, KVH) + partial_bytes(main_grid(), H / KVH) + (step && B > q8::kScanTokens ? q8::store_workspace_bytes(B) : 0) + 256;
+    return ticket_bytes(B, KVH) + partial_bytes(grid(), H / KVH) + (step && B > q8::kScanTokens ? q8::store_workspace_bytes(B) : 0) + 256;
 }
 
 // `step`: the store of a decode step (T = B), or null.
@@ -584,7 +591,7 @@ static int run(const char* who, const DecodeArgs& a, const float* k_scale, const
     p.NB = a.NB;
     p.block_size = a.block_size;
     p.MB = a.MB;
-    p.num_groups = main_grid() / a.KVH;
+    p.num_groups = grid() / a.KVH;
     p.item_cost = kItemCost;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.k_scale = k_scale;
@@ -602,7 +609,7 @@ static int run(const char* who, const DecodeArgs& a, const float* k_scale, const
     const int clear_blocks = (num_tickets + q8::kStoreThreads - 1) / q8::kStoreThreads;
     const bool inside = step && a.B <= q8::kScanTokens;
     if (step && !inside &&
-        (rc = q8::launch_store(who, *step, src_dtype, ws + ticket_bytes(a.B, a.KVH) + partial_bytes(main_grid(), p.G),
+        (rc = q8::launch_store(who, *step, src_dtype, ws + ticket_bytes(a.B, a.KVH) + partial_bytes(grid(), p.G),
                                q8::store_workspace_bytes(a.B), cfg.stream)))
         return rc;
     const int store_blocks = inside ? num_tickets : 0;

@@ -644,30 +644,14 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         for (int e = 0; e < 8; ++e) top = max(top, max(in[e] & 0x7fffu, in[e] >> 16 & 0x7fffu));
 #pragma unroll
                         for (int step = 1; step < 8; step <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
-                        // divided by 2^(e - up): 1.m * 2^(e - 127) becomes 224 < .. <= 448
-                        const uint32_t up = (top & 0x7fu) <= 0x60u ? 8 : 7, e = min(max(top == 0 ? 127u + up : top >> 7, 9u), 254u);
-                        const float down = __uint_as_float((254u + up - e) << 23);
+                        const q8::RowPower power(top);
                         uint32_t hi[4], lo[4];
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            float f[4], g[4];
-#pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                f[2 * h] = __uint_as_float(in[2 * c + h] << 16) * down;
-                                f[2 * h + 1] = __uint_as_float(in[2 * c + h] & 0xffff0000u) * down;
-                            }
-#pragma unroll
-                            for (int h = 0; h < 4; ++h) f[h] = fabsf(f[h]) < INFINITY ? f[h] : __uint_as_float(0x7fffffffu);
-                            const uint32_t h0 = q8::to_e4m3x2(f[0], f[1]), h1 = q8::to_e4m3x2(f[2], f[3]);
-                            const float2 g0 = q8::e4m3x2_to_float2(h0), g1 = q8::e4m3x2_to_float2(h1);
-                            g[0] = f[0] - g0.x, g[1] = f[1] - g0.y, g[2] = f[2] - g1.x, g[3] = f[3] - g1.y;
-                            hi[c] = h0 | h1 << 16;
-                            lo[c] = q8::to_e4m3x2(g[0], g[1]) | q8::to_e4m3x2(g[2], g[3]) << 16;
-                        }
+                        for (int c = 0; c < 4; ++c) q8::split_row(in[2 * c], in[2 * c + 1], power.down, hi[c], lo[c]);
                         uint8_t* to = smem + x * kTileBytes + row * 128 + ((part ^ (row & 7)) << 4);
                         *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                         *reinterpret_cast<uint4*>(to + kByteTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        if (part == 0) sh->q_factor[k & 1][x][row] = __uint_as_float((e - up) << 23);
+                        if (part == 0) sh->q_factor[k & 1][x][row] = power.up;
                     }
                 }
             }
