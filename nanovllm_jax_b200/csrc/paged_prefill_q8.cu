@@ -11,16 +11,18 @@
 //    it.  Twice as many products at twice the rate: the time of the bf16 product, with no conversion of K at all.
 //  * The row's power of two and the K scale of each half of a tile (a scale has 64 slots) go into the factor that the softmax
 //    multiplies its scores by anyway.
-//  * O += P.V stays in bf16: P would lose its small probabilities in e4m3.  A warpgroup of its own turns V bytes into bf16
-//    (value * scale: exact where the scale is a power of two, as the store's are) with rows behind the sequence's end as zeros,
-//    one tile ahead, and splits Q between two items.
+//  * O += P.V runs in fp16 (P would lose its small probabilities in e4m3): e4m3 -> fp16 is exact and one instruction for two
+//    values.  A warpgroup of its own fetches V bytes into its registers a tile ahead, writes fp16 tiles (rows behind the
+//    sequence's end as zeros) and splits Q between two items.  The V scale goes into the exponent of the probabilities, relative
+//    to the unit that O is in: the first tile's scale, moved -- O rescaled, as when the maximum grows -- when a tile's is larger or less
+//    than 2^-kUnitRange of it.  The sums of the probabilities take the exponent back, once per half of a tile.
 //
 // Per CTA (16 warps = 4 warpgroups; registers 64 | 184 | 184 | 80 of the launch's 128 each):
-//   warp 0       TMA producer: K and V bytes, three slots each; the scales of a tile, fetched a tile ahead, into a ring
+//   warp 0       TMA producer: K bytes, four slots; slot and scales of a tile, looked up a tile ahead, into a ring
 //   warps 1, 2   MMA issuers of Q tiles A and B
 //   warp 3       item records
 //   warps 4-11   softmax, as in the bf16 kernel
-//   warps 12-15  Q: bf16 -> two e4m3 tiles and the rows' factors.  V: e4m3 -> bf16, two slots
+//   warps 12-15  Q: bf16 -> two e4m3 tiles and the rows' factors.  V: e4m3 -> fp16, three slots
 // Every mbarrier wait is bounded; on timeout the CTA raises a device error flag, lets its copies land and releases its
 // tensor memory before it exits.
 #include "q8.cuh"
@@ -38,12 +40,11 @@ __device__ int g_error_flag = 0;  // bit 2 (4): a pipeline wait timed out, or no
 
 constexpr int kThreads = 512;
 constexpr int kByteTile = 128 * 128;     // 128 rows of 128 bytes, 128B-swizzled
-constexpr int kSlots = 3;                // of K bytes, and of V bytes
-constexpr int kVSlots = 2;               // of V in bf16
-constexpr int kScales = 8;               // ring of tile scales: nobody is as far ahead of a reader (see the producer)
-constexpr int kK = 2 * kTileBytes;       // offsets: Q (A: hi, lo; B: hi, lo), K, V bytes, V
-constexpr int kVBytes = kK + kSlots * kByteTile;
-constexpr int kV = kVBytes + kSlots * kByteTile;
+constexpr int kSlots = 4;                // of K bytes
+constexpr int kVSlots = 3;               // of V in fp16
+constexpr int kInfos = 8;                // ring of what a tile is: nobody is as far ahead of a reader (see the producer)
+constexpr int kK = 2 * kTileBytes;       // offsets: Q (A: hi, lo; B: hi, lo), K, V
+constexpr int kV = kK + kSlots * kByteTile;
 constexpr int kSmemTiles = kV + kVSlots * kTileBytes;  // 224 KB
 constexpr int kItemRing = 2;
 constexpr int kItemReaders = 3 + 8 + 4;  // TMA producer, two MMA issuers, eight softmax warps, four converting warps
@@ -51,9 +52,14 @@ constexpr int kRegsControl = 64, kRegsSoftmax = 184, kRegsConvert = 80;
 static_assert(kRegsControl + 2 * kRegsSoftmax + kRegsConvert == 4 * 128, "what setmaxnreg asks for is what the launch has");
 
 constexpr float kTiny = 1.17549435e-38f;
+// log2 units: a row's largest probability is 2^kBias, or up to 2^(kBias + kRescaleThreshold) until the maximum moves (fp16: 2^16);
+// one of 2^-21 of it is still a normal fp16 number.
+constexpr float kBias = 7.f;
+constexpr float kUnitRange = 8.f;
 
 struct Source {
     const __nv_bfloat16* q;
+    const uint8_t* v;                // [NB * block_size, KVH, 128] e4m3
     const float *k_scale, *v_scale;  // [NB * block_size / 64, KVH]
     int NB, KVH;
 };
@@ -66,15 +72,15 @@ struct Split : SplitParams {
 
 struct Shared {
     float q_factor[2][2][kTileQ];  // [item parity][Q tile][row]: what a row was divided by
-    float4 scale[kScales];         // of a tile: K first and second half, V first and second half
+    float4 scale[kInfos];          // of a tile: K scales of the first and second half, log2 of the V scales
+    int token[kInfos];             // its first slot
     Item items[kItemRing];         // the items of this CTA, written ahead by warp 3
     uint64_t item_full[kItemRing], item_empty[kItemRing];
     uint64_t q_full, q_empty;
     uint64_t factor_full[2];       // of the item parity: the softmax may come to an item when Q of the next one is there already
     uint64_t k_full[kSlots], k_empty[kSlots];
-    uint64_t vb_full[kSlots], vb_empty[kSlots];  // V bytes
     uint64_t v_full[kVSlots], v_empty[kVSlots];
-    uint64_t scale_full[kScales];
+    uint64_t info_full[kInfos];
     uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
     uint64_t turn[2];  // as in the bf16 kernel
     uint32_t tmem_base;
@@ -99,6 +105,15 @@ __device__ __forceinline__ bool next_item(Shared* sh, uint32_t k, Item& it) {
     return it.n_kv >= 0;
 }
 
+// 16 bytes global -> shared, or zeros.
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // D[tmem] (+)= A[smem] * B[smem], both e4m3, K = 32
 __device__ __forceinline__ void mma_bytes(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -111,6 +126,7 @@ __device__ __forceinline__ void mma_bytes(uint32_t d_tmem, uint64_t a_desc, uint
         : "memory");
 }
 constexpr uint32_t kIdescBytes = (1u << 4) | ((128u >> 4) << 24);  // e4m3 x e4m3 -> fp32, M = 128, both K-major
+constexpr uint32_t kIdescHalf = (1u << 4) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);  // fp16, V MN-major
 constexpr uint32_t idesc_bytes(uint32_t keys) { return kIdescBytes | ((keys >> 3) << 17); }
 
 // One 128-column S row -> running max, optional O rescale, bf16 P in two halves.  DIAG: key column c of this tile is
@@ -121,11 +137,14 @@ constexpr uint32_t idesc_bytes(uint32_t keys) { return kIdescBytes | ((keys >> 3
 // turn_out (or null): where this tile hands over.
 // The whole row is held in registers (the softmax warpgroups raise their register budget with setmaxnreg), so
 // tensor memory is read once and its latency is paid once per tile.
+// c0, c1: factors of the scores of the tile's two halves (positive); the maxima are of the products, in log2 units.
+// v0, v1: log2 of the halves' V scales; unit: log2 of the one that O is in units of.
 template <bool DIAG>
 __device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint32_t t_s, const uint32_t t_o,
                                              const int lim, const int warp_lo, const int warp_hi, const bool first,
                                              const uint32_t o_parity_prev,
-                                             const float c0, const float c1, const uint32_t alive, float& m_run, float& m_used, float& l,
+                                             const float c0, const float c1, const float v0, const float v1, const uint32_t alive, float& m_run,
+                                             float& m_used, float& unit, float& l,
                                              uint64_t* turn_bar, const uint32_t turn_parity, uint64_t* turn_out) {
     uint32_t v[4][32];
     tmem_ld32(t_s, v[0]);
@@ -156,32 +175,36 @@ __device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint
     }
     m_run = max3(m_run, top[0] * c0, top[1] * c1);
     if (turn_bar != nullptr && !wait_or_abort(sh, turn_bar, turn_parity)) return false;
+    const float v_top = fmaxf(v0, v1);
     if (first) {
         m_used = m_run;  // finite for live rows: key 0 of the sequence is visible to every row and sits in the first tile
+        unit = v_top;
     } else {
         const bool grow = m_run - m_used > kRescaleThreshold;
-        if (__ballot_sync(0xffffffffu, grow) & alive) {
-            // O holds sums relative to m_used: bring it to m_run before this tile's P.V is added.
+        const bool other_unit = v_top > unit || v_top < unit - kUnitRange;  // for all rows alike
+        if ((__ballot_sync(0xffffffffu, grow) & alive) || other_unit) {
+            // O holds sums relative to m_used in the old unit: bring it to m_run and the new one before this tile's P.V is added.
             if (!wait_or_abort(sh, &sh->o_full[x], o_parity_prev)) return false;
             tc_fence_after();
             const float f = fast_exp2(m_used - m_run);
+            const float fo = other_unit ? fast_exp2(m_used - m_run + fminf(unit - v_top, 100.f)) : f;
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
                 uint32_t ov[16];
                 tmem_ld16(t_o + c * 16, ov);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+                for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * fo);
                 tmem_st16(t_o + c * 16, ov);
             }
             tmem_wait_st();
             l *= f;
             m_used = m_run;
+            if (other_unit) unit = v_top;
         }
     }
-    // p = 2^(s*scale - m) as bf16 pairs, written over the S columns (all of them are in registers by now):
+    // p = 2^(s*scale - m + the V scale's exponent) as fp16 pairs, written over the S columns (all of them are in registers by now):
     // chunk c (scores 32c..32c+31) becomes packed columns 16c..16c+15.
-    const uint64_t neg2 = pack2(-m_used, -m_used);
     uint64_t acc_a = pack2(0.f, 0.f), acc_b = pack2(0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -189,7 +212,8 @@ __device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[c][i] = 0u;
         } else {
-        const uint64_t scale2 = c < 2 ? pack2(c0, c0) : pack2(c1, c1);
+        const float n = kBias - m_used + ((c < 2 ? v0 : v1) - unit);
+        const uint64_t scale2 = c < 2 ? pack2(c0, c0) : pack2(c1, c1), neg2 = pack2(n, n);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
             float x0, x1, x2, x3;
@@ -200,8 +224,8 @@ __device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint
             const float e2 = fast_exp2(x2), e3 = fast_exp2(x3);
             acc_a = add2(acc_a, pack2(e0, e1));
             acc_b = add2(acc_b, pack2(e2, e3));
-            v[c][i] = pack_bf16(e0, e1);  // in place: word i <= 2i has been consumed
-            v[c][i + 1] = pack_bf16(e2, e3);
+            v[c][i] = pack_half(e0, e1);  // in place: word i <= 2i has been consumed
+            v[c][i + 1] = pack_half(e2, e3);
         }
         }
         tmem_st16(t_s + c * 16, v[c]);
@@ -214,19 +238,19 @@ __device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint
             tc_fence_before();
             __syncwarp();
             if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->p_full[x][c >> 1]);
+            float s0, s1, s2, s3;
+            unpack2(acc_a, s0, s1);
+            unpack2(acc_b, s2, s3);
+            l = fmaf((s0 + s1) + (s2 + s3), fast_exp2(unit - (c < 2 ? v0 : v1)), l);
+            acc_a = acc_b = pack2(0.f, 0.f);
         }
     }
-    float s0, s1, s2, s3;
-    unpack2(acc_a, s0, s1);
-    unpack2(acc_b, s2, s3);
-    l += (s0 + s1) + (s2 + s3);
     return true;
 }
 
 template <class P>
 __global__ void __launch_bounds__(kThreads, 1)
-paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                        const __grid_constant__ P p) {
+paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ P p) {
     extern __shared__ __align__(1024) uint8_t smem[];
     Shared* sh = reinterpret_cast<Shared*>(smem + kSmemTiles);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -248,14 +272,12 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(&sh->k_full[s], 1);
             mbar_init(&sh->k_empty[s], 2);
-            mbar_init(&sh->vb_full[s], 1);
-            mbar_init(&sh->vb_empty[s], 4);
         }
         for (int s = 0; s < kVSlots; ++s) {
             mbar_init(&sh->v_full[s], 4);
             mbar_init(&sh->v_empty[s], 2);
         }
-        for (int s = 0; s < kScales; ++s) mbar_init(&sh->scale_full[s], 1);
+        for (int s = 0; s < kInfos; ++s) mbar_init(&sh->info_full[s], 1);
         for (int x = 0; x < 2; ++x) {
             mbar_init(&sh->s_full[x], 1);
             mbar_init(&sh->p_full[x][0], kTileQ / 32);
@@ -268,7 +290,6 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         sh->tmem_base = 0xFFFFFFFFu;
         fence_mbar_init();
         prefetch_tensormap(&tm_k);
-        prefetch_tensormap(&tm_v);
     }
     __syncthreads();
     if (warp == 1) {
@@ -301,8 +322,8 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 const bool second = it.len_k - j * kTileKV > q8::kGrain;
                 scale.x = __ldg(p.in.k_scale + at);
                 scale.y = second ? __ldg(p.in.k_scale + at + p.in.KVH) : 1.f;
-                scale.z = __ldg(p.in.v_scale + at);
-                scale.w = second ? __ldg(p.in.v_scale + at + p.in.KVH) : 1.f;
+                scale.z = log2f(fmaxf(__ldg(p.in.v_scale + at), kTiny));
+                scale.w = second ? log2f(fmaxf(__ldg(p.in.v_scale + at + p.in.KVH), kTiny)) : scale.z;
             };
             while (ok && next_item(sh, i, it)) {
                 mbar_arrive(&sh->item_empty[i % kItemRing]);
@@ -313,26 +334,19 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     const float4 mine = scale;
                     if (j + 1 < it.n_kv) locate(j + 1);
                     if (!(ok = wait_or_abort(sh, &sh->k_empty[slot], empty))) break;
-                    // Q.K^T(t - 3) is complete, so P.V(t - 4) has been issued: softmax and conversion have read the scales
-                    // of tile t - 4, and those of t - 8 are free to go.
-                    sh->scale[t % kScales] = mine;
-                    mbar_arrive(&sh->scale_full[t % kScales]);
+                    // Q.K^T(t - 4) is complete, so P.V(t - 5) has been issued: softmax and conversion have read what there is
+                    // about tile t - 5, and the entry of t - 8 is free.
+                    sh->scale[t % kInfos] = mine;
+                    sh->token[t % kInfos] = here;
+                    mbar_arrive(&sh->info_full[t % kInfos]);
                     mbar_expect_tx(&sh->k_full[slot], kByteTile);
                     tma_load_3d(smem + kK + slot * kByteTile, &tm_k, &sh->k_full[slot], 0, it.kvh, here);
-                    if (!(ok = wait_or_abort(sh, &sh->vb_empty[slot], empty))) {
-                        (void)mbar_wait(&sh->k_full[slot], (t / kSlots) & 1u, polls_of_ms(90));
-                        break;
-                    }
-                    mbar_expect_tx(&sh->vb_full[slot], kByteTile);
-                    tma_load_3d(smem + kVBytes + slot * kByteTile, &tm_v, &sh->vb_full[slot], 0, it.kvh, here);
                 }
                 ++i;
             }
             if (sh->abort_flag)  // loads in flight land before the memory is released
-                for (uint32_t u = t >= kSlots ? t - kSlots : 0; u < t; ++u) {
+                for (uint32_t u = t >= kSlots ? t - kSlots : 0; u < t; ++u)
                     (void)mbar_wait(&sh->k_full[u % kSlots], (u / kSlots) & 1u, polls_of_ms(90));
-                    (void)mbar_wait(&sh->vb_full[u % kSlots], (u / kSlots) & 1u, polls_of_ms(90));
-                }
         }
     } else if (warp == 3) {
         // ============================== item records ================================
@@ -391,7 +405,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
 #pragma unroll
                     for (int ks = half * 4; ks < half * 4 + 4; ++ks)
                         if (!decltype(last)::value || ks < steps)
-                            mma_ts(o_t, s_t + ks * 8, vd + (uint32_t)((ks * 16 * 128) >> 4), kIdescPV, (j > 0 || ks > 0));
+                            mma_ts(o_t, s_t + ks * 8, vd + (uint32_t)((ks * 16 * 128) >> 4), kIdescHalf, (j > 0 || ks > 0));
                 }
                 ++tiles;
                 return true;
@@ -481,7 +495,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             const int q_pos = it.q0 + x * p.pack.dq;      // first token of this Q tile
             const int first_lim = it.prefix + q_pos;      // last key visible to it
             const int live = min(p.pack.tokens, it.len - q_pos);  // tokens of the tile in front of the sequence's end
-            float m_run = -INFINITY, m_used = -INFINITY, l = 0.f;
+            float m_run = -INFINITY, m_used = -INFINITY, unit = 0.f, l = 0.f;
             if (!(ok = wait_or_abort(sh, &sh->factor_full[k & 1], (k >> 1) & 1u))) break;
             const float factor = sh->q_factor[k & 1][x][row] * p.scale_log2;
             const uint32_t alive = __ballot_sync(0xffffffffu, tok < live);
@@ -490,6 +504,15 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             // kinds run in two separate loops so that each loop body is straight-line code.
             auto tile_step = [&](const int j, auto kind) -> bool {
                 constexpr bool kDiag = decltype(kind)::value == 1, kDead = decltype(kind)::value == 2;
+                float4 scale = {};
+                if constexpr (!kDead) {
+                    const uint32_t t = kt0 + j;
+                    if (!wait_or_abort(sh, &sh->info_full[t % kInfos], (t / kInfos) & 1u)) return false;
+                    scale = sh->scale[t % kInfos];
+                    // at least the smallest normal number: a masked score, -inf, times 0 would be NaN
+                    scale.x = scale.x * factor < kTiny ? kTiny : scale.x * factor;
+                    scale.y = scale.y * factor < kTiny ? kTiny : scale.y * factor;
+                }
                 if (!wait_or_abort(sh, &sh->s_full[x], tiles & 1u)) return false;
                 // A(j) starts after B(j-1); B(j) starts after A(j) while A still has tiles.
                 uint64_t* turn_bar = nullptr;
@@ -512,14 +535,9 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     return true;
                 }
                 const int lim = first_lim - j * kTileKV;
-                const uint32_t t = kt0 + j;
-                if (!wait_or_abort(sh, &sh->scale_full[t % kScales], (t / kScales) & 1u)) return false;
-                const float2 ks = *reinterpret_cast<const float2*>(&sh->scale[t % kScales]);
-                // at least the smallest normal number: a masked score, -inf, times 0 would be NaN
-                const float c0 = ks.x * factor < kTiny ? kTiny : ks.x * factor, c1 = ks.y * factor < kTiny ? kTiny : ks.y * factor;
                 if (!softmax_tile<kDiag>(sh, x, t_s, t_o, kDiag ? lim + min(tok, live - 1) : 0, kDiag ? lim + min(tok_lo, live - 1) : 0,
                                          kDiag ? lim + min(tok_hi, live - 1) : 0, j == 0,
-                                         (tiles - 1) & 1u, c0, c1, alive, m_run, m_used, l, turn_bar, turn_parity,
+                                         (tiles - 1) & 1u, scale.x, scale.y, scale.z, scale.w, alive, m_run, m_used, unit, l, turn_bar, turn_parity,
                                          (both && (x == 0 || j < it.n_a)) ? &sh->turn[x] : nullptr))
                     return false;
                 // the turn is handed over by A after each of its tiles, by B after those that followed one of A's
@@ -539,6 +557,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             // ---- epilogue: O / l -> bf16 -> global, then hand O back to the MMA thread ----
             if (!(ok = wait_or_abort(sh, &sh->o_full[x], (tiles - 1) & 1u))) break;
             tc_fence_after();
+            const float in_units = fast_exp2(unit);
             if constexpr (std::is_same<P, Split>::value) {
                 if (it.kv0 >= 0) {  // a run of a split item: its O, maximum and sum as they are
                     float* part = p.partials + ((size_t)blockIdx.x * 2 + x) * kPartialFloats;
@@ -548,6 +567,8 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                             uint32_t ov[32];
                             tmem_ld32(t_o + c * 32, ov);
                             tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * in_units);
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
                                 *reinterpret_cast<uint4*>(part + row * kD + c * 32 + i * 4) =
@@ -566,7 +587,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     continue;
                 }
             }
-            const float inv = 1.0f / l;
+            const float inv = in_units / l;
             const int head = it.head + x * p.pack.dh + tok_head;
             __nv_bfloat16* orow = p.out + ((size_t)(it.seq_start + q_pos + tok) * p.H + head) * kD;
 #pragma unroll
@@ -616,43 +637,46 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         for (uint32_t k = 0; ok && next_item(sh, k, it); ++k) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh->item_empty[k % kItemRing]);
-            // ---- Q: rows of the item's tiles, those behind the sequence's end as zeros ----
+            // ---- Q: the item's rows, those behind the sequence's end as zeros, split in place: the two halves of a thread's 32 bytes
+            // go where their upper and lower parts will be ----
             if (k > 0 && !(ok = wait_or_abort(sh, &sh->q_empty, (k - 1) & 1u))) break;
-            for (int x = 0; x < (it.n_b > 0 ? 2 : 1); ++x) {
+            const int q_tiles = it.n_b > 0 ? 2 : 1;
+            for (int x = 0; x < q_tiles; ++x) {
                 const int q_pos = it.q0 + x * p.pack.dq, live = min(p.pack.tokens, it.len - q_pos);
-#pragma unroll 1
-                for (int s = 0; s < 8; s += 4) {
-                    uint4 a[4], b[4];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int row = w * 32 + (s + u) * 4 + r4;
-                        const int tok = row / p.pack.heads;
-                        a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
-                        if (tok < live) {
-                            const int head = it.head + x * p.pack.dh + row - tok * p.pack.heads;
-                            const uint4* src = reinterpret_cast<const uint4*>(
-                                p.in.q + ((size_t)(it.seq_start + q_pos + tok) * p.H + head) * kD + part * 16);
-                            a[u] = __ldg(src), b[u] = __ldg(src + 1);
-                        }
-                    }
+                for (int s = 0; s < 8; ++s) {
+                    const int row = w * 32 + s * 4 + r4, tok = row / p.pack.heads;
+                    const int head = it.head + x * p.pack.dh + row - tok * p.pack.heads;
+                    const bool in = tok < live;
+                    const uint4* from = reinterpret_cast<const uint4*>(p.in.q) +
+                                        (in ? ((size_t)(it.seq_start + q_pos + tok) * p.H + head) * (kD / 8) + part * 2 : 0);
+                    const uint32_t to = smem_u32(smem) + x * kTileBytes + row * 128 + ((part ^ (row & 7)) << 4);
+                    copy_16(to, from, in);
+                    copy_16(to + kByteTile, from + 1, in);
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            for (int x = 0; x < q_tiles; ++x) {
+#pragma unroll 2
+                for (int s = 0; s < 8; ++s) {
+                    const int row = w * 32 + s * 4 + r4;
+                    uint4* const at = reinterpret_cast<uint4*>(smem + x * kTileBytes + row * 128 + ((part ^ (row & 7)) << 4));
+                    uint4* const at_lo = at + kByteTile / 16;
+                    const uint4 a = *at, b = *at_lo;
+                    const uint32_t in[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+                    uint32_t top = 0;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int row = w * 32 + (s + u) * 4 + r4;
-                        const uint32_t in[8] = {a[u].x, a[u].y, a[u].z, a[u].w, b[u].x, b[u].y, b[u].z, b[u].w};
-                        uint32_t top = 0;
+                    for (int e = 0; e < 8; ++e) top = __vmaxu2(top, in[e] & 0x7fff7fffu);
+                    top = max(top & 0xffffu, top >> 16);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) top = max(top, max(in[e] & 0x7fffu, in[e] >> 16 & 0x7fffu));
+                    for (int step = 1; step < 8; step <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
+                    const q8::RowPower power(top);
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                        for (int step = 1; step < 8; step <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
-                        const q8::RowPower power(top);
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) q8::split_row(in[2 * c], in[2 * c + 1], power.down, hi[c], lo[c]);
-                        uint8_t* to = smem + x * kTileBytes + row * 128 + ((part ^ (row & 7)) << 4);
-                        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4*>(to + kByteTile) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        if (part == 0) sh->q_factor[k & 1][x][row] = power.up;
-                    }
+                    for (int c = 0; c < 4; ++c) q8::split_row(in[2 * c], in[2 * c + 1], power.down, hi[c], lo[c]);
+                    *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *at_lo = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    if (part == 0) sh->q_factor[k & 1][x][row] = power.up;
                 }
             }
             fence_proxy_async_smem();
@@ -661,44 +685,41 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 mbar_arrive(&sh->factor_full[k & 1]);
                 mbar_arrive(&sh->q_full);
             }
-            // ---- V, tile by tile ----
-            for (int j = 0; j < it.n_kv; ++j, ++t) {
-                const int slot = t % kSlots, vs = t % kVSlots, own = it.len_k - j * kTileKV;
-                if (!(ok = wait_or_abort(sh, &sh->scale_full[t % kScales], (t / kScales) & 1u))) break;
-                const float scale = w < 2 ? sh->scale[t % kScales].z : sh->scale[t % kScales].w;
-                if (!(ok = wait_or_abort(sh, &sh->vb_full[slot], (t / kSlots) & 1u))) break;
-                const uint8_t* from = smem + kVBytes + slot * kByteTile + (w * 32 + r4) * 128;
-                uint4 in[8];
+            // ---- V, tile by tile: the bytes of the next one are on their way while this one is written ----
+            uint4 in[8];
+            auto fetch = [&](int j) {
+                if (!wait_or_abort(sh, &sh->info_full[t % kInfos], (t / kInfos) & 1u)) return false;
+                const int own = it.len_k - j * kTileKV;
+                const uint8_t* from = p.in.v + ((size_t)(sh->token[t % kInfos] + w * 32 + r4) * p.in.KVH + it.kvh) * kD + part * 16;
 #pragma unroll
-                for (int s = 0; s < 8; ++s) in[s] = *reinterpret_cast<const uint4*>(from + s * 512 + ((part ^ ((s * 4 + r4) & 7)) << 4));
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh->vb_empty[slot]);
+                for (int s = 0; s < 8; ++s) {
+                    in[s] = make_uint4(0u, 0u, 0u, 0u);  // behind the sequence's end: 0 * garbage would poison the row
+                    if (w * 32 + s * 4 + r4 < own) in[s] = __ldg(reinterpret_cast<const uint4*>(from + (size_t)s * 4 * p.in.KVH * kD));
+                }
+                return true;
+            };
+            ok = fetch(0);
+            for (int j = 0; ok && j < it.n_kv; ++j) {
+                const int vs = t % kVSlots;
                 if (!(ok = wait_or_abort(sh, &sh->v_empty[vs], ((t / kVSlots) & 1u) ^ 1u))) break;
                 uint8_t* to = smem + kV + vs * kTileBytes + (part >> 2) * kPanelBytes + (w * 32 + r4) * 128;
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {
-                    const uint32_t b[4] = {in[s].x, in[s].y, in[s].z, in[s].w};
-                    uint32_t o[8];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const float2 f = q8::e4m3x2_to_float2(b[c] & 0xffffu), g = q8::e4m3x2_to_float2(b[c] >> 16);
-                        o[2 * c] = pack_bf16(f.x * scale, f.y * scale);
-                        o[2 * c + 1] = pack_bf16(g.x * scale, g.y * scale);
-                    }
-                    if (w * 32 + s * 4 + r4 >= own) {  // behind the sequence's end: 0 * garbage would poison the row
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) o[c] = 0u;
-                    }
+                    const uint4 lo = make_uint4(q8::e4m3x2_to_half2(in[s].x & 0xffffu), q8::e4m3x2_to_half2(in[s].x >> 16),
+                                                q8::e4m3x2_to_half2(in[s].y & 0xffffu), q8::e4m3x2_to_half2(in[s].y >> 16));
+                    const uint4 hi = make_uint4(q8::e4m3x2_to_half2(in[s].z & 0xffffu), q8::e4m3x2_to_half2(in[s].z >> 16),
+                                                q8::e4m3x2_to_half2(in[s].w & 0xffffu), q8::e4m3x2_to_half2(in[s].w >> 16));
                     // Dims 16 part .. + 15 are chunks 2 (part % 4) and + 1 of a panel's row.  Lanes of the second panel take
                     // theirs in the other order, so that eight lanes always write eight different banks' chunks.
                     const int r7 = (s * 4 + r4) & 7, first = 2 * (part & 3) + (part >> 2), second = first ^ 1;
-                    const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
                     *reinterpret_cast<uint4*>(to + s * 512 + ((first ^ r7) << 4)) = part < 4 ? lo : hi;
                     *reinterpret_cast<uint4*>(to + s * 512 + ((second ^ r7) << 4)) = part < 4 ? hi : lo;
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh->v_full[vs]);
+                ++t;
+                if (j + 1 < it.n_kv) ok = fetch(j + 1);
             }
         }
     }
@@ -752,22 +773,21 @@ int launch_bytes(const Params& p, const SplitParams* split, const Bytes& in, con
     using namespace prefill_q8;
     int rc = ensure_attr();
     if (rc) return rc;
-    CUtensorMap tm_k, tm_v;
+    CUtensorMap tm_k;
     if ((rc = make_byte_map(&tm_k, k, KVH, slots))) return rc;
-    if ((rc = make_byte_map(&tm_v, v, KVH, slots))) return rc;
-    const Source src = {(const __nv_bfloat16*)q, in.k_scale, in.v_scale, in.NB, KVH};
+    const Source src = {(const __nv_bfloat16*)q, (const uint8_t*)v, in.k_scale, in.v_scale, in.NB, KVH};
     cfg.blockDim = dim3(prefill_q8::kThreads);
     cfg.dynamicSmemBytes = prefill_q8::kSmemBytes;
     if (split) {
         Split s;
         static_cast<SplitParams&>(s) = *split;
         s.in = src;
-        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_prefill_q8_kernel<Split>, tm_k, tm_v, s));
+        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_prefill_q8_kernel<Split>, tm_k, s));
     } else {
         Whole s;
         static_cast<Params&>(s) = p;
         s.in = src;
-        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_prefill_q8_kernel<Whole>, tm_k, tm_v, s));
+        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_prefill_q8_kernel<Whole>, tm_k, s));
     }
     return NVLLM_B200_OK;
 }

@@ -76,13 +76,15 @@ def dequantised(values, scales):
 def attention(q, k, v, tables, len_q, len_k, scale, block):
     """Causal attention of the last len_q[b] tokens of every sequence over its len_k[b] tokens in the pages.
 
-    q [sum len_q, H, 128]; k, v [NB, block, KVH, 128].  Returns (out, weight, score): weight = sum p |v| / sum p and score = the
-    largest sum |q||k| scale of a row, by which errors are bounded.  A sequence without keys gives zeros.
+    q [sum len_q, H, 128]; k, v [NB, block, KVH, 128].  Returns (out, weight, score, small), the last three for bounds of errors:
+    weight = sum p |v|; score = the largest sum |q||k| scale of a row; small = sum min(p |v|, 2^-21 p16 |v| + 2^-31 max p max |v|)
+    with p16 the largest p of a token's sixteen: what probabilities that underflow in fp16 may cost.  A sequence without keys gives
+    zeros.
     """
     t, h, d = q.shape
     nb, kvh = k.shape[0], k.shape[2]
     g = h // kvh
-    out, weight, score = np.zeros((t, h, d)), np.zeros((t, h, d)), np.zeros((t, h, 1))
+    out, weight, small, score = np.zeros((t, h, d)), np.zeros((t, h, d)), np.zeros((t, h, d)), np.zeros((t, h, 1))
     row = 0
     for b in range(len(len_q)):
         n = int(len_k[b])
@@ -98,10 +100,13 @@ def attention(q, k, v, tables, len_q, len_k, scale, block):
                     p = np.exp(s - s.max())
                     p /= p.sum()
                     out[row, head] = p @ vh
-                    weight[row, head] = p @ np.abs(vh)
+                    av = np.abs(vh)
+                    weight[row, head] = p @ av
+                    p16 = np.repeat(np.pad(p, (0, -seen % 16)).reshape(-1, 16).max(1), 16)[:seen]
+                    small[row, head] = np.minimum(p[:, None] * av, (2.0 ** -21 * p16)[:, None] * av + 2.0 ** -31 * p.max() * av.max()).sum(0)
                     score[row, head] = (np.abs(kh) @ np.abs(qr)).max() * abs(scale)
             row += 1
-    return out, weight, score
+    return out, weight, score, small
 
 
 def copy_pages(caches, src, dst, block, tokens=None, tables=None):

@@ -44,12 +44,12 @@ def test_attention_is_softmax():
     rng = np.random.default_rng(2)
     k, v = rng.normal(size=(2, 3, 64, 1, 128))
     q = rng.normal(size=(2, 2, 128))
-    out, weight, score = cache8.attention(q, k, v, [[2, 0]], [2], [100], 0.1, 64)
+    out, weight, score, small = cache8.attention(q, k, v, [[2, 0]], [2], [100], 0.1, 64)
     kk, vv = np.concatenate([k[2], k[0]])[:, 0], np.concatenate([v[2], v[0]])[:, 0]
     for i, n in enumerate((99, 100)):
         p = torch.softmax(torch.from_numpy(q[i] @ kk[:n].T * 0.1), -1)
         assert np.allclose(out[i], p.numpy() @ vv[:n], rtol=0, atol=1e-13)
-    assert (np.abs(out) <= weight + 1e-15).all() and (score > 0).all()
+    assert (np.abs(out) <= weight + 1e-15).all() and (score > 0).all() and (small <= weight).all()
 
 
 def test_copy_pages():
