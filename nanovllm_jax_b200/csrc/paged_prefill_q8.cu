@@ -42,6 +42,7 @@ constexpr int kThreads = 512;
 constexpr int kByteTile = 128 * 128;     // 128 rows of 128 bytes, 128B-swizzled
 constexpr int kSlots = 4;                // of K bytes
 constexpr int kVSlots = 3;               // of V in fp16
+constexpr int kStep = 64;                // keys of a softmax step: half a K/V tile, a block of scales
 constexpr int kInfos = 8;                // ring of what a tile is: nobody is as far ahead of a reader (see the producer)
 constexpr int kK = 2 * kTileBytes;       // offsets: Q (A: hi, lo; B: hi, lo), K, V
 constexpr int kV = kK + kSlots * kByteTile;
@@ -81,8 +82,8 @@ struct Shared {
     uint64_t k_full[kSlots], k_empty[kSlots];
     uint64_t v_full[kVSlots], v_empty[kVSlots];
     uint64_t info_full[kInfos];
-    uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
-    uint64_t turn[2];  // as in the bf16 kernel
+    uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [Q tile][step parity]
+    uint64_t o_empty[2];
     uint32_t tmem_base;
     volatile int abort_flag;
 };
@@ -129,32 +130,28 @@ constexpr uint32_t kIdescBytes = (1u << 4) | ((128u >> 4) << 24);  // e4m3 x e4m
 constexpr uint32_t kIdescHalf = (1u << 4) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);  // fp16, V MN-major
 constexpr uint32_t idesc_bytes(uint32_t keys) { return kIdescBytes | ((keys >> 3) << 17); }
 
-// One 128-column S row -> running max, optional O rescale, bf16 P in two halves.  DIAG: key column c of this tile is
-// visible iff c <= lim (lim may be negative -- nothing visible in this tile -- or >= 127), and the limits of the warp's rows
-// lie in warp_lo .. warp_hi; columns behind every limit may hold anything.  alive: the warp's rows in front of the
-// sequence's end; the others (the next sequence's queries, rows that no load fills) have no vote on when to rescale, or the
-// live rows' bits would depend on them.  turn_bar (or null): the other tile's hand-over this tile's exponentials wait for;
-// turn_out (or null): where this tile hands over.
-// The whole row is held in registers (the softmax warpgroups raise their register budget with setmaxnreg), so
-// tensor memory is read once and its latency is paid once per tile.
-// c0, c1: factors of the scores of the tile's two halves (positive); the maxima are of the products, in log2 units.
-// v0, v1: log2 of the halves' V scales; unit: log2 of the one that O is in units of.
+// Steps of Q tile x in an item, and how many keys its last one has (of the item's last row).
+__device__ __forceinline__ int keys_of(const Params& p, const Item& it, int x, int n_x) { return min(visible_keys(p, it, x), n_x * kTileKV); }
+__device__ __forceinline__ int steps_of(int keys) { return (keys + kStep - 1) / kStep; }
+
+// One step of a row: 64 scores -> running maximum, perhaps O rescaled, fp16 P over the first half of the scores' columns.
+// DIAG: key c of this step is visible iff c <= lim (which may be negative, or 63 and more), and the limits of the warp's rows
+// lie in warp_lo .. warp_hi; keys behind every limit may hold anything.  alive: the warp's rows in front of the sequence's
+// end; the others have no vote on when to rescale, or the live rows' bits would depend on them.
+// c0: factor of the scores (positive); the maxima are of the products, in log2 units.  v0: log2 of the V scale; unit: of the one
+// that O is in units of.  o_bar: the P.V in front of this step's.
 template <bool DIAG>
-__device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint32_t t_s, const uint32_t t_o,
-                                             const int lim, const int warp_lo, const int warp_hi, const bool first,
-                                             const uint32_t o_parity_prev,
-                                             const float c0, const float c1, const float v0, const float v1, const uint32_t alive, float& m_run,
-                                             float& m_used, float& unit, float& l,
-                                             uint64_t* turn_bar, const uint32_t turn_parity, uint64_t* turn_out) {
-    uint32_t v[4][32];
+__device__ __forceinline__ bool softmax_step(Shared* sh, const uint32_t t_s, const uint32_t t_o, const int lim, const int warp_lo,
+                                             const int warp_hi, const bool first, uint64_t* o_bar, const uint32_t o_parity, const float c0,
+                                             const float v0, const uint32_t alive, float& m_run, float& m_used, float& unit, float& l,
+                                             uint64_t* p_bar) {
+    uint32_t v[2][32];
     tmem_ld32(t_s, v[0]);
     tmem_ld32(t_s + 32, v[1]);
-    tmem_ld32(t_s + 64, v[2]);
-    tmem_ld32(t_s + 96, v[3]);
     tmem_wait_ld();
-    float top[2] = {-INFINITY, -INFINITY};  // of the two halves
+    float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < 2; ++c) {
         if (DIAG) {
             if (32 * c > warp_hi) continue;  // nothing of this chunk is visible to any row of the warp
             if (32 * c + 31 > warp_lo) {     // mask in place so that the second pass needs no select
@@ -163,7 +160,6 @@ __device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint
                     if (c * 32 + i > lim) v[c][i] = 0xFF800000u;
             }
         }
-        float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 32; i += 8) {
             mx0 = max3(mx0, __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
@@ -171,23 +167,20 @@ __device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint
             mx2 = max3(mx2, __uint_as_float(v[c][i + 4]), __uint_as_float(v[c][i + 5]));
             mx3 = max3(mx3, __uint_as_float(v[c][i + 6]), __uint_as_float(v[c][i + 7]));
         }
-        top[c >> 1] = max3(top[c >> 1], fmaxf(mx0, mx1), fmaxf(mx2, mx3));
     }
-    m_run = max3(m_run, top[0] * c0, top[1] * c1);
-    if (turn_bar != nullptr && !wait_or_abort(sh, turn_bar, turn_parity)) return false;
-    const float v_top = fmaxf(v0, v1);
+    m_run = fmaxf(m_run, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c0);
     if (first) {
-        m_used = m_run;  // finite for live rows: key 0 of the sequence is visible to every row and sits in the first tile
-        unit = v_top;
+        m_used = m_run;  // finite for live rows: key 0 of the sequence is visible to every row and sits in the first step
+        unit = v0;
     } else {
         const bool grow = m_run - m_used > kRescaleThreshold;
-        const bool other_unit = v_top > unit || v_top < unit - kUnitRange;  // for all rows alike
+        const bool other_unit = v0 > unit || v0 < unit - kUnitRange;  // for all rows alike
         if ((__ballot_sync(0xffffffffu, grow) & alive) || other_unit) {
-            // O holds sums relative to m_used in the old unit: bring it to m_run and the new one before this tile's P.V is added.
-            if (!wait_or_abort(sh, &sh->o_full[x], o_parity_prev)) return false;
+            // O holds sums relative to m_used in the old unit: bring it to m_run and the new one before this step's P.V is added.
+            if (!wait_or_abort(sh, o_bar, o_parity)) return false;
             tc_fence_after();
             const float f = fast_exp2(m_used - m_run);
-            const float fo = other_unit ? fast_exp2(m_used - m_run + fminf(unit - v_top, 100.f)) : f;
+            const float fo = other_unit ? fast_exp2(m_used - m_run + fminf(unit - v0, 100.f)) : f;
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
                 uint32_t ov[16];
@@ -200,51 +193,43 @@ __device__ __forceinline__ bool softmax_tile(Shared* sh, const int x, const uint
             tmem_wait_st();
             l *= f;
             m_used = m_run;
-            if (other_unit) unit = v_top;
+            if (other_unit) unit = v0;
         }
     }
-    // p = 2^(s*scale - m + the V scale's exponent) as fp16 pairs, written over the S columns (all of them are in registers by now):
-    // chunk c (scores 32c..32c+31) becomes packed columns 16c..16c+15.
+    // p = 2^(s*c0 - m + the V scale's exponent) as fp16 pairs, written over the S columns (all of them are in registers by
+    // now): chunk c (scores 32c .. 32c + 31) becomes packed columns 16c .. 16c + 15.
+    const float n = kBias - m_used + (v0 - unit);
+    const uint64_t scale2 = pack2(c0, c0), neg2 = pack2(n, n);
     uint64_t acc_a = pack2(0.f, 0.f), acc_b = pack2(0.f, 0.f);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < 2; ++c) {
         if (DIAG && 32 * c > warp_hi) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) v[c][i] = 0u;
         } else {
-        const float n = kBias - m_used + ((c < 2 ? v0 : v1) - unit);
-        const uint64_t scale2 = c < 2 ? pack2(c0, c0) : pack2(c1, c1), neg2 = pack2(n, n);
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            float x0, x1, x2, x3;
-            unpack2(fma2(pack2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), scale2, neg2), x0, x1);
-            unpack2(fma2(pack2(__uint_as_float(v[c][2 * i + 2]), __uint_as_float(v[c][2 * i + 3])), scale2, neg2), x2,
-                    x3);
-            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);  // 2^-inf = 0 for masked keys
-            const float e2 = fast_exp2(x2), e3 = fast_exp2(x3);
-            acc_a = add2(acc_a, pack2(e0, e1));
-            acc_b = add2(acc_b, pack2(e2, e3));
-            v[c][i] = pack_half(e0, e1);  // in place: word i <= 2i has been consumed
-            v[c][i + 1] = pack_half(e2, e3);
-        }
+            for (int i = 0; i < 16; i += 2) {
+                float x0, x1, x2, x3;
+                unpack2(fma2(pack2(__uint_as_float(v[c][2 * i]), __uint_as_float(v[c][2 * i + 1])), scale2, neg2), x0, x1);
+                unpack2(fma2(pack2(__uint_as_float(v[c][2 * i + 2]), __uint_as_float(v[c][2 * i + 3])), scale2, neg2), x2, x3);
+                const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);  // 2^-inf = 0 for masked keys
+                const float e2 = fast_exp2(x2), e3 = fast_exp2(x3);
+                acc_a = add2(acc_a, pack2(e0, e1));
+                acc_b = add2(acc_b, pack2(e2, e3));
+                v[c][i] = pack_half(e0, e1);  // in place: word i <= 2i has been consumed
+                v[c][i + 1] = pack_half(e2, e3);
+            }
         }
         tmem_st16(t_s + c * 16, v[c]);
-        if (c == 3 && turn_out != nullptr) {
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0) mbar_arrive(turn_out);
-        }
-        if (c & 1) {  // a half of P (64 keys) is complete: release its four P.V k-steps
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0) mbar_arrive(&sh->p_full[x][c >> 1]);
-            float s0, s1, s2, s3;
-            unpack2(acc_a, s0, s1);
-            unpack2(acc_b, s2, s3);
-            l = fmaf((s0 + s1) + (s2 + s3), fast_exp2(unit - (c < 2 ? v0 : v1)), l);
-            acc_a = acc_b = pack2(0.f, 0.f);
-        }
     }
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(p_bar);
+    float s0, s1, s2, s3;
+    unpack2(acc_a, s0, s1);
+    unpack2(acc_b, s2, s3);
+    l = fmaf((s0 + s1) + (s2 + s3), fast_exp2(unit - v0), l);
     return true;
 }
 
@@ -279,12 +264,12 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         }
         for (int s = 0; s < kInfos; ++s) mbar_init(&sh->info_full[s], 1);
         for (int x = 0; x < 2; ++x) {
-            mbar_init(&sh->s_full[x], 1);
-            mbar_init(&sh->p_full[x][0], kTileQ / 32);
-            mbar_init(&sh->p_full[x][1], kTileQ / 32);
-            mbar_init(&sh->o_full[x], 1);
+            for (int b = 0; b < 2; ++b) {
+                mbar_init(&sh->s_full[x][b], 1);
+                mbar_init(&sh->p_full[x][b], kTileQ / 32);
+                mbar_init(&sh->o_done[x][b], 1);
+            }
             mbar_init(&sh->o_empty[x], kTileQ / 32);
-            mbar_init(&sh->turn[x], kTileQ / 32);
         }
         sh->abort_flag = 0;
         sh->tmem_base = 0xFFFFFFFFu;
@@ -373,93 +358,73 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         }
     } else {
         // ============================== MMA issuers ===============================
-        // As in the bf16 kernel: one issuing thread per Q tile, K(j+1) awaited before P.V(j) is issued, all commits of the
-        // pair behind Q.K^T(j+1); a tile's last products leave out the keys behind every row.
+        // One issuing thread per Q tile.  S has two buffers of a step each: Q.K^T of step h + 2 is issued right behind P.V of step h,
+        // whose P it overwrites (a thread's MMAs run in order), so the scores of a step are there before the softmax of the one in
+        // front of it is done.  The last step's products leave out the keys behind every row.
         if (lane == 0) {
             const int x = warp - 1;
             const uint32_t s_t = tmem + x * 128, o_t = tmem + 256 + x * 128;
             const uint64_t q_desc = make_desc(smem_u32(smem + x * kTileBytes), 16, 1024);
             const uint64_t k_desc0 = make_desc(smem_u32(smem + kK), 16, 1024), v_desc0 = mnmajor_desc(smem_u32(smem + kV), 0);
-            uint32_t kt = 0;     // K/V tiles consumed before this item
-            uint32_t tiles = 0;  // tiles finished by this Q tile, over all items (barrier phases)
-            uint32_t used = 0;   // items in which this Q tile was active (o_empty phases)
-            uint32_t i = 0;      // items
+            uint32_t kt = 0;    // K/V tiles consumed before this item
+            uint32_t g = 0;     // steps of this Q tile before this item (buffers and barrier phases)
+            uint32_t used = 0;  // items in which this Q tile was active (o_empty phases)
+            uint32_t i = 0;     // items
             bool ok = true;
-
-            auto issue_qk = [&](uint64_t kd, bool behind_pv, uint32_t idesc) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half)  // the two tiles that Q is the sum of
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        mma_bytes(s_t, q_desc + (uint32_t)((half * kByteTile + ks * 32) >> 4), kd + (uint32_t)((ks * 32) >> 4), idesc,
-                                  half + ks > 0);
-                if (behind_pv) tc_commit(&sh->o_full[x]);
-                tc_commit(&sh->s_full[x]);
-            };
-            auto issue_pv = [&](int j, uint64_t vd, auto last, int steps) -> bool {
-                if (j == 0 && used > 0 && !wait_or_abort(sh, &sh->o_empty[x], (used - 1) & 1u)) return false;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (!wait_or_abort(sh, &sh->p_full[x][half], tiles & 1u)) return false;
-                    tc_fence_after();
-#pragma unroll
-                    for (int ks = half * 4; ks < half * 4 + 4; ++ks)
-                        if (!decltype(last)::value || ks < steps)
-                            mma_ts(o_t, s_t + ks * 8, vd + (uint32_t)((ks * 16 * 128) >> 4), kIdescHalf, (j > 0 || ks > 0));
-                }
-                ++tiles;
-                return true;
-            };
             auto k_full = [&](uint32_t t) { return wait_or_abort(sh, &sh->k_full[t % kSlots], (t / kSlots) & 1u); };
-            auto k_desc = [&](uint32_t t) { return k_desc0 + (t % kSlots) * (uint32_t)(kByteTile >> 4); };
-
-            const std::false_type full;
-            const std::true_type last;
+            auto v_full = [&](uint32_t t) { return wait_or_abort(sh, &sh->v_full[t % kVSlots], (t / kVSlots) & 1u); };
             Item it;
             while (ok && next_item(sh, i, it)) {
                 mbar_arrive(&sh->item_empty[i % kItemRing]);
-                const int n_x = x == 0 ? it.n_a : it.n_b;
-                const int steps = key_steps(visible_keys(p, it, x), n_x);  // of the last tile
-                const uint32_t idesc_last = idesc_bytes(16 * steps);
+                const int n_x = x == 0 ? it.n_a : it.n_b, keys = keys_of(p, it, x, n_x), steps = n_x > 0 ? steps_of(keys) : 0;
+                const int last = (keys - (steps - 1) * kStep + 15) >> 4;  // 16-key parts of the last step that hold any
                 if (!(ok = wait_or_abort(sh, &sh->q_full, i & 1u))) break;
-                if (n_x == 0) mbar_arrive(&sh->q_empty);  // this tile never reads the Q buffer of this item
-                if (!(ok = k_full(kt))) break;
-                if (n_x > 0) {
+                auto qk = [&](int h) -> bool {
+                    const uint32_t t = kt + (h >> 1), b = (g + h) & 1u;
+                    if (!k_full(t)) return false;
                     tc_fence_after();
-                    issue_qk(k_desc(kt), false, n_x > 1 ? idesc_bytes(kTileKV) : idesc_last);
-                    tc_commit(&sh->k_empty[kt % kSlots]);
-                    if (n_x == 1) tc_commit(&sh->q_empty);
-                } else {
-                    mbar_arrive(&sh->k_empty[kt % kSlots]);
+                    const uint64_t kd = k_desc0 + (t % kSlots) * (uint32_t)(kByteTile >> 4) + (h & 1) * (uint32_t)(kStep * 128 >> 4);
+                    const uint32_t idesc = idesc_bytes(h + 1 < steps ? kStep : 16 * last);
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)  // the two tiles that Q is the sum of
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            mma_bytes(s_t + b * kStep, q_desc + (uint32_t)((part * kByteTile + ks * 32) >> 4), kd + (uint32_t)((ks * 32) >> 4),
+                                      idesc, part + ks > 0);
+                    tc_commit(&sh->s_full[x][b]);
+                    if ((h & 1) || h + 1 == steps) tc_commit(&sh->k_empty[t % kSlots]);
+                    if (h + 1 == steps) tc_commit(&sh->q_empty);
+                    return true;
+                };
+                if (steps == 0) mbar_arrive(&sh->q_empty);  // this tile never reads the Q buffer of this item
+                if (steps > 0) ok = qk(0);
+                if (ok && steps > 1) ok = qk(1);
+                for (int h = 0; ok && h < steps; ++h) {
+                    const uint32_t t = kt + (h >> 1), b = (g + h) & 1u;
+                    if (!(ok = v_full(t))) break;
+                    if (h == 0 && used > 0 && !(ok = wait_or_abort(sh, &sh->o_empty[x], (used - 1) & 1u))) break;
+                    if (!(ok = wait_or_abort(sh, &sh->p_full[x][b], ((g + h) >> 1) & 1u))) break;
+                    tc_fence_after();
+                    const uint64_t vd = v_desc0 + (t % kVSlots) * (uint32_t)(kTileBytes >> 4) + (h & 1) * (uint32_t)(kStep * 128 >> 4);
+                    const int parts = h + 1 < steps ? 4 : last;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        if (ks < parts)
+                            mma_ts(o_t, s_t + b * kStep + ks * 8, vd + (uint32_t)((ks * 16 * 128) >> 4), kIdescHalf, (h > 0 || ks > 0));
+                    tc_commit(&sh->o_done[x][b]);
+                    if ((h & 1) || h + 1 == steps) tc_commit(&sh->v_empty[t % kVSlots]);
+                    if (h + 2 < steps) ok = qk(h + 2);
                 }
-                for (int j = 0; ok && j < it.n_kv; ++j) {
-                    const uint32_t t = kt + j, vs = t % kVSlots;
-                    if (!(ok = wait_or_abort(sh, &sh->v_full[vs], (t / kVSlots) & 1u))) break;
-                    if (j + 1 < it.n_kv && !(ok = k_full(t + 1))) break;
-                    if (j < n_x) {
-                        const uint64_t vd = v_desc0 + vs * (uint32_t)(kTileBytes >> 4);
-                        if (j + 1 < n_x) {
-                            if (!(ok = issue_pv(j, vd, full, 8))) break;
-                        } else {
-                            if (!(ok = issue_pv(j, vd, last, steps))) break;
-                            tc_commit(&sh->o_full[x]);
-                            tc_commit(&sh->v_empty[vs]);
-                        }
-                    } else {
-                        mbar_arrive(&sh->v_empty[vs]);
-                    }
-                    if (j + 1 < it.n_kv) {
-                        if (j + 1 < n_x) {
-                            issue_qk(k_desc(t + 1), true, j + 2 < n_x ? idesc_bytes(kTileKV) : idesc_last);
-                            tc_commit(&sh->k_empty[(t + 1) % kSlots]);
-                            tc_commit(&sh->v_empty[vs]);
-                            if (j + 2 == n_x) tc_commit(&sh->q_empty);  // this tile's last Q.K^T has been issued
-                        } else {
-                            mbar_arrive(&sh->k_empty[(t + 1) % kSlots]);
-                        }
-                    }
+                // tiles that only the other Q tile has steps in
+                for (int j = (steps + 1) >> 1; ok && j < it.n_kv; ++j) {
+                    const uint32_t t = kt + j;
+                    if (!(ok = k_full(t))) break;
+                    mbar_arrive(&sh->k_empty[t % kSlots]);
+                    if (!(ok = v_full(t))) break;
+                    mbar_arrive(&sh->v_empty[t % kVSlots]);
                 }
-                used += n_x > 0 ? 1 : 0;
+                g += steps;
+                used += steps > 0 ? 1 : 0;
                 kt += it.n_kv;
                 ++i;
             }
@@ -476,22 +441,21 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const uint32_t t_s = tmem + x * 128 + lane_base;
         const uint32_t t_o = tmem + 256 + x * 128 + lane_base;
-        uint32_t tiles = 0;  // tiles finished by this Q tile over all items (barrier phases)
-        uint32_t turns_seen = 0;  // completions of the other tile's turn barrier this warp has consumed
-        uint32_t kt = 0;          // K/V tiles of the items before this one
+        uint32_t g = 0;   // steps of this Q tile in the items before this one (buffers and barrier phases)
+        uint32_t kt = 0;  // K/V tiles of the items before this one
         bool ok = true;
         Item it;
         for (uint32_t k = 0; ok && next_item(sh, k, it); ++k) {
             const int n_x = x == 0 ? it.n_a : it.n_b;
-            const uint32_t kt0 = kt;
+            const uint32_t kt0 = kt, g0 = g;
             kt += it.n_kv;
             if (n_x == 0) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh->item_empty[k % kItemRing]);
                 continue;
             }
-            // The two tiles take turns, as in the bf16 kernel.
-            const bool both = it.n_b > 0 && it.n_a > 1;
+            const int steps = steps_of(keys_of(p, it, x, n_x));
+            g += steps;
             const int q_pos = it.q0 + x * p.pack.dq;      // first token of this Q tile
             const int first_lim = it.prefix + q_pos;      // last key visible to it
             const int live = min(p.pack.tokens, it.len - q_pos);  // tokens of the tile in front of the sequence's end
@@ -499,63 +463,43 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             if (!(ok = wait_or_abort(sh, &sh->factor_full[k & 1], (k >> 1) & 1u))) break;
             const float factor = sh->q_factor[k & 1][x][row] * p.scale_log2;
             const uint32_t alive = __ballot_sync(0xffffffffu, tok < live);
-            // One KV tile of this Q tile.  Tiles whose last key the tile's first row may still see need no mask; the
-            // one or two after them (one when the prefix is a multiple of the tile) are masked per element.  The two
+            // Steps whose last key the tile's first row may still see need no mask; the others are masked per element.  The two
             // kinds run in two separate loops so that each loop body is straight-line code.
-            auto tile_step = [&](const int j, auto kind) -> bool {
+            auto step = [&](const int h, auto kind) -> bool {
                 constexpr bool kDiag = decltype(kind)::value == 1, kDead = decltype(kind)::value == 2;
-                float4 scale = {};
+                const uint32_t t = kt0 + (h >> 1), b = (g0 + h) & 1u, phase = ((g0 + h) >> 1) & 1u;
+                float c0 = 0.f, v0 = 0.f;
                 if constexpr (!kDead) {
-                    const uint32_t t = kt0 + j;
                     if (!wait_or_abort(sh, &sh->info_full[t % kInfos], (t / kInfos) & 1u)) return false;
-                    scale = sh->scale[t % kInfos];
-                    // at least the smallest normal number: a masked score, -inf, times 0 would be NaN
-                    scale.x = scale.x * factor < kTiny ? kTiny : scale.x * factor;
-                    scale.y = scale.y * factor < kTiny ? kTiny : scale.y * factor;
+                    const float* scale = &sh->scale[t % kInfos].x + (h & 1);
+                    c0 = scale[0] * factor, v0 = scale[2];
+                    c0 = c0 < kTiny ? kTiny : c0;  // a normal number: a masked score, -inf, times 0 would be NaN
                 }
-                if (!wait_or_abort(sh, &sh->s_full[x], tiles & 1u)) return false;
-                // A(j) starts after B(j-1); B(j) starts after A(j) while A still has tiles.
-                uint64_t* turn_bar = nullptr;
-                const uint32_t turn_parity = turns_seen & 1u;
-                if (both && (x == 0 ? j >= 1 : j < it.n_a)) {
-                    turn_bar = &sh->turn[x ^ 1];
-                    ++turns_seen;
-                }
+                if (!wait_or_abort(sh, &sh->s_full[x][b], phase)) return false;
                 tc_fence_after();
-                if constexpr (kDead) {  // nothing but the hand-overs: P and O of these rows may hold anything
-                    if (turn_bar != nullptr && !wait_or_abort(sh, turn_bar, turn_parity)) return false;
+                if constexpr (kDead) {  // nothing but the hand-over: P and O of these rows may hold anything
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) {
-                        if (both && (x == 0 || j < it.n_a)) mbar_arrive(&sh->turn[x]);
-                        mbar_arrive(&sh->p_full[x][0]);
-                        mbar_arrive(&sh->p_full[x][1]);
-                    }
-                    ++tiles;
+                    if (lane == 0) mbar_arrive(&sh->p_full[x][b]);
                     return true;
                 }
-                const int lim = first_lim - j * kTileKV;
-                if (!softmax_tile<kDiag>(sh, x, t_s, t_o, kDiag ? lim + min(tok, live - 1) : 0, kDiag ? lim + min(tok_lo, live - 1) : 0,
-                                         kDiag ? lim + min(tok_hi, live - 1) : 0, j == 0,
-                                         (tiles - 1) & 1u, scale.x, scale.y, scale.z, scale.w, alive, m_run, m_used, unit, l, turn_bar, turn_parity,
-                                         (both && (x == 0 || j < it.n_a)) ? &sh->turn[x] : nullptr))
-                    return false;
-                // the turn is handed over by A after each of its tiles, by B after those that followed one of A's
-                ++tiles;
-                return true;
+                const int lim = first_lim - h * kStep;
+                return softmax_step<kDiag>(sh, t_s + b * kStep, t_o, kDiag ? lim + min(tok, live - 1) : 0, kDiag ? lim + min(tok_lo, live - 1) : 0,
+                                           kDiag ? lim + min(tok_hi, live - 1) : 0, h == 0, &sh->o_done[x][b ^ 1], ((g0 + h - 1) >> 1) & 1u, c0,
+                                           v0, alive, m_run, m_used, unit, l, &sh->p_full[x][b]);
             };
-            const int n_plain = min(n_x, (first_lim + 1) / kTileKV);  // tiles j with j * 128 + 127 <= first_lim
-            int j = 0;
+            const int n_plain = min(steps, (first_lim + 1) / kStep);  // steps h with 64 h + 63 <= first_lim
+            int h = 0;
             const bool dead = tok_lo >= live;  // the whole warp lies behind the sequence's last row
             if (dead) {
-                for (; ok && j < n_x; ++j) ok = tile_step(j, std::integral_constant<int, 2>{});
+                for (; ok && h < steps; ++h) ok = step(h, std::integral_constant<int, 2>{});
             } else {
-                for (; ok && j < n_plain; ++j) ok = tile_step(j, std::integral_constant<int, 0>{});
-                for (; ok && j < n_x; ++j) ok = tile_step(j, std::integral_constant<int, 1>{});
+                for (; ok && h < n_plain; ++h) ok = step(h, std::integral_constant<int, 0>{});
+                for (; ok && h < steps; ++h) ok = step(h, std::integral_constant<int, 1>{});
             }
             if (!ok) break;
             // ---- epilogue: O / l -> bf16 -> global, then hand O back to the MMA thread ----
-            if (!(ok = wait_or_abort(sh, &sh->o_full[x], (tiles - 1) & 1u))) break;
+            if (!(ok = wait_or_abort(sh, &sh->o_done[x][(g - 1) & 1u], ((g - 1) >> 1) & 1u))) break;
             tc_fence_after();
             const float in_units = fast_exp2(unit);
             if constexpr (std::is_same<P, Split>::value) {
@@ -583,7 +527,6 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                         mbar_arrive(&sh->o_empty[x]);
                         mbar_arrive(&sh->item_empty[k % kItemRing]);
                     }
-                    if (x == 0 && both) ok = wait_or_abort(sh, &sh->turn[1], turns_seen++ & 1u);
                     continue;
                 }
             }
@@ -623,9 +566,6 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 mbar_arrive(&sh->o_empty[x]);
                 mbar_arrive(&sh->item_empty[k % kItemRing]);  // only now: the next claim waits for it
             }
-            // B's last turn.  Else A, two hand-overs further with the next item's first tile, could lap a warp of B that was
-            // held up in front of its last wait (2.7 us would do), and the parity would alias.
-            if (x == 0 && both) ok = wait_or_abort(sh, &sh->turn[1], turns_seen++ & 1u);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsConvert));
