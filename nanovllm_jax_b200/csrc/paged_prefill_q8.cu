@@ -17,7 +17,7 @@
 //    to the unit that O is in: the first tile's scale, moved -- O rescaled, as when the maximum grows -- when a tile's is larger or less
 //    than 2^-kUnitRange of it.  The sums of the probabilities take the exponent back, once per half of a tile.
 //
-// Per CTA (16 warps = 4 warpgroups; registers 64 | 184 | 184 | 80 of the launch's 128 each):
+// Per CTA (16 warps = 4 warpgroups; registers 96 | 160 | 160 | 96 of the launch's 128 each):
 //   warp 0       TMA producer: K bytes, four slots; slot and scales of a tile, looked up a tile ahead, into a ring
 //   warps 1, 2   MMA issuers of Q tiles A and B
 //   warp 3       item records
@@ -49,7 +49,7 @@ constexpr int kV = kK + kSlots * kByteTile;
 constexpr int kSmemTiles = kV + kVSlots * kTileBytes;  // 224 KB
 constexpr int kItemRing = 2;
 constexpr int kItemReaders = 3 + 8 + 4;  // TMA producer, two MMA issuers, eight softmax warps, four converting warps
-constexpr int kRegsControl = 64, kRegsSoftmax = 184, kRegsConvert = 80;
+constexpr int kRegsControl = 96, kRegsSoftmax = 160, kRegsConvert = 96;
 static_assert(kRegsControl + 2 * kRegsSoftmax + kRegsConvert == 4 * 128, "what setmaxnreg asks for is what the launch has");
 
 constexpr float kTiny = 1.17549435e-38f;
@@ -199,6 +199,7 @@ __device__ __forceinline__ bool softmax_step(Shared* sh, const uint32_t t_s, con
     // p = 2^(s*c0 - m + the V scale's exponent) as fp16 pairs, written over the S columns (all of them are in registers by
     // now): chunk c (scores 32c .. 32c + 31) becomes packed columns 16c .. 16c + 15.
     const float n = kBias - m_used + (v0 - unit);
+    const float back = fast_exp2(unit - v0);
     const uint64_t scale2 = pack2(c0, c0), neg2 = pack2(n, n);
     uint64_t acc_a = pack2(0.f, 0.f), acc_b = pack2(0.f, 0.f);
 #pragma unroll
@@ -229,7 +230,7 @@ __device__ __forceinline__ bool softmax_step(Shared* sh, const uint32_t t_s, con
     float s0, s1, s2, s3;
     unpack2(acc_a, s0, s1);
     unpack2(acc_b, s2, s3);
-    l = fmaf((s0 + s1) + (s2 + s3), fast_exp2(unit - v0), l);
+    l = fmaf((s0 + s1) + (s2 + s3), back, l);
     return true;
 }
 
@@ -465,16 +466,17 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             const uint32_t alive = __ballot_sync(0xffffffffu, tok < live);
             // Steps whose last key the tile's first row may still see need no mask; the others are masked per element.  The two
             // kinds run in two separate loops so that each loop body is straight-line code.
+            float4 scale = {};
             auto step = [&](const int h, auto kind) -> bool {
                 constexpr bool kDiag = decltype(kind)::value == 1, kDead = decltype(kind)::value == 2;
                 const uint32_t t = kt0 + (h >> 1), b = (g0 + h) & 1u, phase = ((g0 + h) >> 1) & 1u;
-                float c0 = 0.f, v0 = 0.f;
-                if constexpr (!kDead) {
+                if (!kDead && (h & 1) == 0) {  // what the tile is, for its two steps
                     if (!wait_or_abort(sh, &sh->info_full[t % kInfos], (t / kInfos) & 1u)) return false;
-                    const float* scale = &sh->scale[t % kInfos].x + (h & 1);
-                    c0 = scale[0] * factor, v0 = scale[2];
-                    c0 = c0 < kTiny ? kTiny : c0;  // a normal number: a masked score, -inf, times 0 would be NaN
+                    scale = sh->scale[t % kInfos];
                 }
+                float c0 = ((h & 1) ? scale.y : scale.x) * factor;
+                c0 = c0 < kTiny ? kTiny : c0;  // a normal number: a masked score, -inf, times 0 would be NaN
+                const float v0 = (h & 1) ? scale.w : scale.z;
                 if (!wait_or_abort(sh, &sh->s_full[x][b], phase)) return false;
                 tc_fence_after();
                 if constexpr (kDead) {  // nothing but the hand-over: P and O of these rows may hold anything
