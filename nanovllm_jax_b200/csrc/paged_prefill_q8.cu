@@ -82,7 +82,8 @@ struct Shared {
     uint64_t k_full[kSlots], k_empty[kSlots];
     uint64_t v_full[kVSlots], v_empty[kVSlots];
     uint64_t info_full[kInfos];
-    uint64_t s_full[2][2], p_full[2][2], o_done[2][2];  // [Q tile][step parity]
+    uint64_t s_full[2][2], p_full[2][2];  // [Q tile][step parity]
+    uint64_t o_done[2][2];               // [Q tile][an item's last step but one (or only one), its last one]
     uint64_t o_empty[2];
     uint32_t tmem_base;
     volatile int abort_flag;
@@ -257,7 +258,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         mbar_init(&sh->factor_full[1], 4);
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(&sh->k_full[s], 1);
-            mbar_init(&sh->k_empty[s], 2);
+            mbar_init(&sh->k_empty[s], 2);  // from each Q tile: its softmax, or its issuer where it has no step there
         }
         for (int s = 0; s < kVSlots; ++s) {
             mbar_init(&sh->v_full[s], 4);
@@ -361,7 +362,10 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         // ============================== MMA issuers ===============================
         // One issuing thread per Q tile.  S has two buffers of a step each: Q.K^T of step h + 2 is issued right behind P.V of step h,
         // whose P it overwrites (a thread's MMAs run in order), so the scores of a step are there before the softmax of the one in
-        // front of it is done.  The last step's products leave out the keys behind every row.
+        // front of it is done, and with S(h + 2) there P.V(h) is complete as well: only an item's last two are committed by
+        // themselves.  A poll and a commit cost this thread about a hundred cycles each, so a K slot is given back by a softmax
+        // warp and a tile is waited for once (2048 tokens x 32 heads behind 16384 keys: 655 -> 640 us).
+        // The last step's products leave out the keys behind every row.
         if (lane == 0) {
             const int x = warp - 1;
             const uint32_t s_t = tmem + x * 128, o_t = tmem + 256 + x * 128;
@@ -382,7 +386,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 if (!(ok = wait_or_abort(sh, &sh->q_full, i & 1u))) break;
                 auto qk = [&](int h) -> bool {
                     const uint32_t t = kt + (h >> 1), b = (g + h) & 1u;
-                    if (!k_full(t)) return false;
+                    if ((h & 1) == 0 && !k_full(t)) return false;
                     tc_fence_after();
                     const uint64_t kd = k_desc0 + (t % kSlots) * (uint32_t)(kByteTile >> 4) + (h & 1) * (uint32_t)(kStep * 128 >> 4);
                     const uint32_t idesc = idesc_bytes(h + 1 < steps ? kStep : 16 * last);
@@ -393,7 +397,6 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                             mma_bytes(s_t + b * kStep, q_desc + (uint32_t)((part * kByteTile + ks * 32) >> 4), kd + (uint32_t)((ks * 32) >> 4),
                                       idesc, part + ks > 0);
                     tc_commit(&sh->s_full[x][b]);
-                    if ((h & 1) || h + 1 == steps) tc_commit(&sh->k_empty[t % kSlots]);
                     if (h + 1 == steps) tc_commit(&sh->q_empty);
                     return true;
                 };
@@ -402,7 +405,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 if (ok && steps > 1) ok = qk(1);
                 for (int h = 0; ok && h < steps; ++h) {
                     const uint32_t t = kt + (h >> 1), b = (g + h) & 1u;
-                    if (!(ok = v_full(t))) break;
+                    if ((h & 1) == 0 && !(ok = v_full(t))) break;
                     if (h == 0 && used > 0 && !(ok = wait_or_abort(sh, &sh->o_empty[x], (used - 1) & 1u))) break;
                     if (!(ok = wait_or_abort(sh, &sh->p_full[x][b], ((g + h) >> 1) & 1u))) break;
                     tc_fence_after();
@@ -412,7 +415,8 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     for (int ks = 0; ks < 4; ++ks)
                         if (ks < parts)
                             mma_ts(o_t, s_t + b * kStep + ks * 8, vd + (uint32_t)((ks * 16 * 128) >> 4), kIdescHalf, (h > 0 || ks > 0));
-                    tc_commit(&sh->o_done[x][b]);
+                    if (h + 2 == steps || steps == 1) tc_commit(&sh->o_done[x][0]);
+                    if (h + 1 == steps) tc_commit(&sh->o_done[x][1]);
                     if ((h & 1) || h + 1 == steps) tc_commit(&sh->v_empty[t % kVSlots]);
                     if (h + 2 < steps) ok = qk(h + 2);
                 }
@@ -444,6 +448,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         const uint32_t t_o = tmem + 256 + x * 128 + lane_base;
         uint32_t g = 0;   // steps of this Q tile in the items before this one (buffers and barrier phases)
         uint32_t kt = 0;  // K/V tiles of the items before this one
+        uint32_t used = 0;  // of them, those in which this Q tile was active
         bool ok = true;
         Item it;
         for (uint32_t k = 0; ok && next_item(sh, k, it); ++k) {
@@ -479,6 +484,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 const float v0 = (h & 1) ? scale.w : scale.z;
                 if (!wait_or_abort(sh, &sh->s_full[x][b], phase)) return false;
                 tc_fence_after();
+                if (((h & 1) || h + 1 == steps) && quarter == 0 && lane == 0) mbar_arrive(&sh->k_empty[t % kSlots]);
                 if constexpr (kDead) {  // nothing but the hand-over: P and O of these rows may hold anything
                     tc_fence_before();
                     __syncwarp();
@@ -487,7 +493,8 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 }
                 const int lim = first_lim - h * kStep;
                 return softmax_step<kDiag>(sh, t_s + b * kStep, t_o, kDiag ? lim + min(tok, live - 1) : 0, kDiag ? lim + min(tok_lo, live - 1) : 0,
-                                           kDiag ? lim + min(tok_hi, live - 1) : 0, h == 0, &sh->o_done[x][b ^ 1], ((g0 + h - 1) >> 1) & 1u, c0,
+                                           kDiag ? lim + min(tok_hi, live - 1) : 0, h == 0, h + 1 < steps ? &sh->s_full[x][b ^ 1] : &sh->o_done[x][0],
+                                           h + 1 < steps ? ((g0 + h + 1) >> 1) & 1u : used & 1u, c0,
                                            v0, alive, m_run, m_used, unit, l, &sh->p_full[x][b]);
             };
             const int n_plain = min(steps, (first_lim + 1) / kStep);  // steps h with 64 h + 63 <= first_lim
@@ -501,8 +508,9 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             }
             if (!ok) break;
             // ---- epilogue: O / l -> bf16 -> global, then hand O back to the MMA thread ----
-            if (!(ok = wait_or_abort(sh, &sh->o_done[x][(g - 1) & 1u], ((g - 1) >> 1) & 1u))) break;
+            if (!(ok = wait_or_abort(sh, &sh->o_done[x][1], used & 1u))) break;
             tc_fence_after();
+            ++used;
             const float in_units = fast_exp2(unit);
             if constexpr (std::is_same<P, Split>::value) {
                 if (it.kv0 >= 0) {  // a run of a split item: its O, maximum and sum as they are
