@@ -502,7 +502,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
                 *reinterpret_cast<float4*>(part + r * kD + c8) = a;
                 *reinterpret_cast<float4*>(part + r * kD + c8 + 4) = b;
                 if (c8 == 0) {
-                    part[p.G * kD + r] = mt;
+                    part[p.G * kD + r] = mt == -INFINITY ? 0.f : mt;  // only where all scores are NaN, and then o is: not to be left out
                     part[p.G * kD + kMaxG + r] = lt;
                 }
             }

@@ -196,6 +196,27 @@ def test_nan_stays_in_its_sequence():
     assert out[0].isnan().all() and out[1].isfinite().all()
 
 
+@pytest.mark.parametrize("n", (40, 9000))
+def test_nan_query_and_nan_keys(n):
+    """A head whose scores are all NaN gives NaN, in one run of keys or in many; so does a run whose keys all are."""
+    import torch
+    from nanovllm_jax_b200 import ops
+    rng = np.random.default_rng(n)
+    q, tables, ctx, nb = make(rng, [n, n], 4, 2, 64)
+    cache = random_cache(rng, nb, 64, 2)
+    clean = ops.paged_decode_q8(q, *cache, tables, ctx, 0.09, 64)
+    q[0, 1] = float("nan")
+    out = ops.paged_decode_q8(q, *cache, tables, ctx, 0.09, 64)
+    assert out[0, 1].isnan().all()
+    out[0, 1] = clean[0, 1]
+    assert torch.equal(out, clean)
+    q[0, 1] = 0
+    pages = tables[1, :min(20, -(-n // 64))].long()
+    cache[0].view(torch.uint8)[pages, :, 1] = 0x7F
+    out = ops.paged_decode_q8(q, *cache, tables, ctx, 0.09, 64)
+    assert out[1, 2:].isnan().all() and out[1, :2].isfinite().all() and out[0].isfinite().all()
+
+
 def test_cache_beyond_4_gb():
     """Offsets of the last pages pass 32 bits: 5 GB of keys, 8 kv heads, a sequence in the first and the last pages."""
     import torch
