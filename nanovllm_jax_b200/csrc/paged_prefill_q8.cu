@@ -57,6 +57,9 @@ constexpr float kTiny = 1.17549435e-38f;
 // one of 2^-21 of it is still a normal fp16 number.
 constexpr float kBias = 7.f;
 constexpr float kUnitRange = 8.f;
+// A V scale below 2^-kScaleRange of the largest one before it in the run counts as that (a block of zeros has the least scale there
+// is): its values are nothing beside what p * v may be off by, and O, in units of it, would leave fp32.
+constexpr float kScaleRange = 64.f;
 
 struct Source {
     const __nv_bfloat16* q;
@@ -181,7 +184,7 @@ __device__ __forceinline__ bool softmax_step(Shared* sh, const uint32_t t_s, con
             if (!wait_or_abort(sh, o_bar, o_parity)) return false;
             tc_fence_after();
             const float f = fast_exp2(m_used - m_run);
-            const float fo = other_unit ? fast_exp2(m_used - m_run + fminf(unit - v0, 100.f)) : f;
+            const float fo = other_unit ? fast_exp2(m_used - m_run + (unit - v0)) : f;
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
                 uint32_t ov[16];
@@ -300,6 +303,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             Item it = {};
             int token = 0;
             float4 scale;
+            float least = 0.f;  // log2 of the smallest V scale that counts
             // First slot of K/V tile j and its scales: one per 64 slots, of which the second may lie behind the last key.
             auto locate = [&](int j) {
                 const int off = (max(it.kv0, 0) + j) * kTileKV;
@@ -311,6 +315,10 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 scale.y = second ? __ldg(p.in.k_scale + at + p.in.KVH) : 1.f;
                 scale.z = log2f(fmaxf(__ldg(p.in.v_scale + at), kTiny));
                 scale.w = second ? log2f(fmaxf(__ldg(p.in.v_scale + at + p.in.KVH), kTiny)) : scale.z;
+                if (j > 0) scale.z = fmaxf(scale.z, least);
+                least = j > 0 ? fmaxf(least, scale.z - kScaleRange) : scale.z - kScaleRange;
+                scale.w = fmaxf(scale.w, least);
+                least = fmaxf(least, scale.w - kScaleRange);
             };
             while (ok && next_item(sh, i, it)) {
                 mbar_arrive(&sh->item_empty[i % kItemRing]);

@@ -208,3 +208,40 @@ def test_refusals():
     small = random_cache(rng, 2, 64, 2)
     with pytest.raises(RuntimeError, match="multiple of 128"):
         call(k=small[0], v=small[1], ks=small[2], vs=small[3], b=64)
+
+
+@pytest.mark.parametrize("exponents", [(-117, 0, 0), (0, -117, 0, -117, -117), (-60, 40, -117, 0, -30), (40, -117, -60)])
+@pytest.mark.parametrize("pre", (0, 700, 6000))
+def test_value_scales_far_apart(exponents, pre):
+    """Blocks of zeros, whose scale is the least there is, between others; and values of any magnitude next to one another."""
+    import torch
+    from nanovllm_jax_b200 import _lib, ops
+    rng = np.random.default_rng(pre + len(exponents))
+    q, tables, cu, cu_k, _, nb, lens = make(rng, [200, 9], [pre, 3], 4, 1, 128)
+    cache = random_cache(rng, nb, 128, 1)
+    of = torch.tensor(exponents)
+    for b in range(2):
+        for i, page in enumerate(tables[b, :-(-lens[b] // 128)].tolist()):
+            for half in range(2):
+                e = int(of[(2 * i + half) % len(exponents)])
+                cache[3][page, half] = 2.0 ** e
+                if e == -117 and exponents[0] <= 0:
+                    cache[1].view(torch.uint8)[page, 64 * half:64 * half + 64] = 0
+    out = ops.paged_prefill_q8(q, *cache, tables, cu, cu_k, 200, 0.09, 128)
+    close(out, expect(q, cache, tables, [200, 9], lens, 0.09, 128), q, 0.09, key_size(cache))
+    assert _lib.device_status() == 0
+
+
+def test_nan_query_of_a_split_sequence():
+    import torch
+    from nanovllm_jax_b200 import ops
+    rng = np.random.default_rng(9)
+    q, tables, cu, cu_k, _, nb, _ = make(rng, [5], [6000], 8, 1, 128)
+    cache = random_cache(rng, nb, 128, 1)
+    clean = ops.paged_prefill_q8(q, *cache, tables, cu, cu_k, 5, 0.09, 128)
+    q[2, 3] = float("nan")
+    out = ops.paged_prefill_q8(q, *cache, tables, cu, cu_k, 5, 0.09, 128)
+    assert out[2, 3].isnan().all()
+    q[2, 3] = 0
+    out[2, 3] = clean[2, 3]
+    assert torch.equal(out, clean)
