@@ -27,6 +27,8 @@
  *     Anything else returns NVLLM_B200_EUNSUPPORTED -- there is no fallback path.
  *   - Thread safety: re-entrant; calls may come from any host thread; work is
  *     ordered by the stream it is enqueued on.
+ *   - A workspace belongs to one call until the call's work is complete: calls, or replays of
+ *     captured graphs, that may overlap on the GPU need one each.
  */
 #ifndef NVLLM_B200_ATTN_H_
 #define NVLLM_B200_ATTN_H_

@@ -15,7 +15,9 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -136,27 +138,88 @@ float to_float(PyObject* o) {
 
 // One scratch buffer per (device, stream), grown on demand: calls on one stream are ordered, so they may share it.  At
 // most kMaxWorkspaces buffers are kept; the one used longest ago goes back to torch's allocator first (it was allocated
-// on its own stream, so the allocator hands it out again only behind that stream's work).  A buffer that a stream capture
-// has seen is never given back: the graph refers to it for as long as it may be replayed.  Used under the GIL.
+// on its own stream, so the allocator hands it out again only behind that stream's work).  Used under the GIL.
+// A stream capture has buffers of its own, one per stream in it: its graph may be replayed on any stream, beside other graphs
+// that were captured on the same one.  The graph holds them and gives them back when it is destroyed.
 struct Workspace {
     int device;
     cudaStream_t stream;
     uint64_t used;
-    bool captured;
     at::Tensor buf;
 };
 constexpr size_t kMaxWorkspaces = 64;
-std::vector<at::Tensor>& captured_buffers() {
-    static auto* list = new std::vector<at::Tensor>();
-    return *list;
-}
 std::vector<Workspace>& workspaces() {
     static auto* list = new std::vector<Workspace>();  // never destroyed: the allocator may be gone at exit
     return *list;
 }
 uint64_t workspace_clock = 0;
 
+struct Captured {
+    unsigned long long id;  // of the capture
+    int device;
+    cudaStream_t stream;
+    at::Tensor buf;
+};
+std::vector<Captured*>& captured() {
+    static auto* list = new std::vector<Captured*>();
+    return *list;
+}
+// Those whose graph is gone.  The call-back runs on a thread of the driver's, which may not call back into it.
+std::mutex& given_back_mutex() {
+    static auto* m = new std::mutex();
+    return *m;
+}
+std::vector<Captured*>& given_back() {
+    static auto* list = new std::vector<Captured*>();
+    return *list;
+}
+std::atomic<bool> any_given_back{false};
+void CUDART_CB give_back(void* c) {
+    const std::lock_guard<std::mutex> lock(given_back_mutex());
+    given_back().push_back(static_cast<Captured*>(c));
+    any_given_back = true;
+}
+void release_given_back() {
+    std::vector<Captured*> gone;
+    {
+        const std::lock_guard<std::mutex> lock(given_back_mutex());
+        gone.swap(given_back());
+        any_given_back = false;
+    }
+    for (Captured* c : gone) {
+        auto& list = captured();
+        list.erase(std::remove(list.begin(), list.end(), c), list.end());
+        delete c;
+    }
+}
+at::Tensor new_buffer(int device, size_t nbytes) {
+    return at::empty({(int64_t)std::max(nbytes, (size_t)1 << 20)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
+}
+
+const at::Tensor& captured_workspace(unsigned long long id, cudaGraph_t graph, int device, cudaStream_t stream, size_t nbytes) {
+    for (Captured* c : captured())
+        if (c->id == id && c->stream == stream && c->device == device && (size_t)c->buf.numel() >= nbytes) return c->buf;
+    auto* c = new Captured{id, device, stream, new_buffer(device, nbytes)};
+    captured().push_back(c);
+    cudaUserObject_t object;
+    if (cudaUserObjectCreate(&object, c, give_back, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) {
+        (void)cudaGetLastError();  // then it is kept for good
+    } else if (cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess) {
+        (void)cudaGetLastError();
+    }
+    return c->buf;
+}
+
 const at::Tensor& workspace(int device, cudaStream_t stream, size_t nbytes) {
+    if (any_given_back) release_given_back();
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    if (cudaStreamGetCaptureInfo(stream, &status, &id, &graph) != cudaSuccess) {
+        (void)cudaGetLastError();
+        status = cudaStreamCaptureStatusNone;
+    }
+    if (status == cudaStreamCaptureStatusActive) return captured_workspace(id, graph, device, stream, nbytes);
     auto& list = workspaces();
     Workspace* w = nullptr;
     for (auto& e : list)
@@ -165,8 +228,7 @@ const at::Tensor& workspace(int device, cudaStream_t stream, size_t nbytes) {
             break;
         }
     if (!w || (size_t)w->buf.numel() < nbytes) {
-        const int64_t n = (int64_t)std::max(nbytes, (size_t)1 << 20);
-        at::Tensor buf = at::empty({n}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
+        at::Tensor buf = new_buffer(device, nbytes);
         if (!w) {
             if (list.size() < kMaxWorkspaces) {
                 list.push_back(Workspace{});
@@ -177,18 +239,11 @@ const at::Tensor& workspace(int device, cudaStream_t stream, size_t nbytes) {
                     if (e.used < w->used) w = &e;
             }
         }
-        if (w->captured) captured_buffers().push_back(w->buf);
         w->device = device;
         w->stream = stream;
-        w->captured = false;
         w->buf = std::move(buf);
     }
     w->used = ++workspace_clock;
-    if (!w->captured) {
-        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) (void)cudaGetLastError();
-        w->captured = status != cudaStreamCaptureStatusNone;
-    }
     return w->buf;
 }
 

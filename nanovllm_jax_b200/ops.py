@@ -18,7 +18,8 @@ from . import _lib
 def workspace(device, nbytes: int) -> torch.Tensor:
     """A cached scratch buffer of at least ``nbytes`` on ``device`` (grown on demand, never shrunk).
 
-    One buffer per (device, stream): calls on one stream are ordered, so they may share it.
+    One buffer per (device, stream): calls on one stream are ordered, so they may share it.  Calls that a stream capture records get
+    buffers of the graph's own, which may be replayed on any stream; it holds them until it is destroyed.
     """
     index = torch.device(device).index
     return _lib.binding().workspace(torch.cuda.current_device() if index is None else index, nbytes)
