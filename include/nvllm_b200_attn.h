@@ -395,8 +395,10 @@ int nvllm_b200_decode_step_q8(const void* q, const void* k, const void* v, void*
  * paged_prefill_q8: nvllm_b200_paged_prefill over an 8-bit cache (block_size a multiple of 128); the arguments they share, the
  * workspace and the device status bits mean the same.  The new tokens' rows must have been stored already.
  * Math: scores in fp32 from the cache's own values and from q as the sum of two e4m3 numbers under a power of two per row (exact
- * for components above 2^-11 of the row's largest, to within 2^-18 of it for smaller ones); bf16 probabilities and bf16
- * value * scale (exact for scales that are powers of two) into the P.V product with fp32 accumulation.
+ * for components above 2^-11 of the row's largest, to within 2^-18 of it for smaller ones); fp16 probabilities, which carry the V
+ * scale, times the cache's own values in fp16 (exact) into fp32.  What a probability loses by underflow is relative to the row's
+ * largest one and to the largest V scale among the keys before it: at most 2^-32 of their product times 448; a V scale below 2^-64 of that
+ * one counts as 2^-64 of it.
  */
 int nvllm_b200_paged_prefill_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
                                 const float* v_scale, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,

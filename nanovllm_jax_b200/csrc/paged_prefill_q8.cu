@@ -17,6 +17,17 @@
 //    to the unit that O is in: the first tile's scale, moved -- O rescaled, as when the maximum grows -- when a tile's is larger or less
 //    than 2^-kUnitRange of it.  The sums of the probabilities take the exponent back, once per half of a tile.
 //
+// Softmax steps are of 64 keys, with two score buffers per Q tile; a step's P lies over its own scores.
+//
+// What bounds it, at 2048 tokens x 32 heads behind 16384 keys (640 us; 585 GFLOP, 352 us at the measured bf16 rate; the bf16 kernel
+// takes 520, and 256 items on 148 SMs cost either an eighth): the MMAs and the chain from a step's scores to its P.V.  A
+// 128 x 64 x 32 byte product reads 6 KB of shared memory, 48 cycles for 32 of arithmetic.  Left out one by one (wrong results, to see
+// what counts): the lower part of Q 575 us, three quarters of P.V 555, both and the rest of Q.K^T 520; the exponentials 641 and
+// without all of the products 408; the conversion 636; the V loads 627.
+// Measured instead: V bytes staged by TMA and written as bf16 668 (12 sequences of 17..700 tokens behind 500..5000: 303, now 254);
+// steps of 128 keys and one score buffer 638 (276); the next step's scores taken into registers before this one's exponentials 767
+// (324); sixteen softmax warps, two threads a row 707 (291); a share of the exponentials as polynomials 686 (an eighth) .. 744 (a quarter).
+//
 // Per CTA (16 warps = 4 warpgroups; registers 96 | 160 | 160 | 96 of the launch's 128 each):
 //   warp 0       TMA producer: K bytes, four slots; slot and scales of a tile, looked up a tile ahead, into a ring
 //   warps 1, 2   MMA issuers of Q tiles A and B

@@ -11,6 +11,10 @@
 //    wait only then; a run that is alone under its hash goes ahead, of others the first of a block takes the rows of all.
 //    (CTAs that look through all slots themselves, while their rows are on their way, are no better in between: 48 prompts of
 //    5..300 tokens, fp32, 2 kv heads: 11.1 us, with the kernel in front 9.6.)
+//
+// Measured: 16 prompts of 128..4096 tokens, 8 kv heads, bf16: 42.3 us, 4.9 TB/s, 0.76 of a plain copy's rate (loads in flight and issue
+// slots, 0.6 of which are taken, share the bound; asking for the window's rows before its slots are known: 43.6; 128 tokens a CTA:
+// 44.9); 64 appended rows 4 to 5 us.
 #include "store_kvcache_q8.cuh"
 
 #include <algorithm>
