@@ -606,15 +606,16 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         for (uint32_t k = 0; ok && next_item(sh, k, it); ++k) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh->item_empty[k % kItemRing]);
-            // ---- Q: the item's rows, those behind the sequence's end as zeros, split in place: the two halves of a thread's 32 bytes
-            // go where their upper and lower parts will be ----
+            // ---- Q: the item's rows, split in place: the two halves of a thread's 32 bytes go where their upper and lower parts will
+            // be.  Sixteen rows at a time over the warps, those behind the sequence's end left out: they hold anything, and so do their
+            // scores (five drafted tokens of sequences of 16 / 2 heads: a run waited 5 us for 128 rows by 32 a warp, two for 40) ----
             if (k > 0 && !(ok = wait_or_abort(sh, &sh->q_empty, (k - 1) & 1u))) break;
             const int q_tiles = it.n_b > 0 ? 2 : 1;
             for (int x = 0; x < q_tiles; ++x) {
                 const int q_pos = it.q0 + x * p.pack.dq, live = min(p.pack.tokens, it.len - q_pos);
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {
-                    const int row = w * 32 + s * 4 + r4, tok = row / p.pack.heads;
+                    const int row = s * 16 + w * 4 + r4, tok = row / p.pack.heads;
                     const int head = it.head + x * p.pack.dh + row - tok * p.pack.heads;
                     const bool in = tok < live;
                     const uint4* from = reinterpret_cast<const uint4*>(p.in.q) +
@@ -626,9 +627,11 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             for (int x = 0; x < q_tiles; ++x) {
+                const int live = min(p.pack.tokens, it.len - (it.q0 + x * p.pack.dq));
+                const int groups = min(8, (live * p.pack.heads + 15) >> 4);  // of 16 rows, that hold live ones
 #pragma unroll 2
-                for (int s = 0; s < 8; ++s) {
-                    const int row = w * 32 + s * 4 + r4;
+                for (int s = 0; s < groups; ++s) {
+                    const int row = s * 16 + w * 4 + r4;
                     uint4* const at = reinterpret_cast<uint4*>(smem + x * kTileBytes + row * 128 + ((part ^ (row & 7)) << 4));
                     uint4* const at_lo = at + kByteTile / 16;
                     const uint4 a = *at, b = *at_lo;
@@ -641,8 +644,13 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     for (int step = 1; step < 8; step <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
                     const q8::RowPower power(top);
                     uint32_t hi[4], lo[4];
+                    if (__any_sync(0xffffffffu, top >= 0x7f80u)) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) q8::split_row(in[2 * c], in[2 * c + 1], power.down, hi[c], lo[c]);
+                        for (int c = 0; c < 4; ++c) q8::split_row<true>(in[2 * c], in[2 * c + 1], power.down, hi[c], lo[c]);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) q8::split_row<false>(in[2 * c], in[2 * c + 1], power.down, hi[c], lo[c]);
+                    }
                     *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *at_lo = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     if (part == 0) sh->q_factor[k & 1][x][row] = power.up;
