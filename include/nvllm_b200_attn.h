@@ -400,6 +400,7 @@ int nvllm_b200_decode_step_q8(const void* q, const void* k, const void* v, void*
  * largest one and to the largest V scale among the keys before it: at most 2^-32 of their product times 448; a V scale below 2^-64 of that
  * one counts as 2^-64 of it.
  */
+size_t nvllm_b200_paged_prefill_q8_workspace_bytes(int64_t T, int B, int H, int KVH, int D);
 int nvllm_b200_paged_prefill_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
                                 const float* v_scale, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                                 const int32_t* block_tables, const int32_t* cu_seqlens_q_host, void* out, void* workspace,

@@ -48,6 +48,7 @@ SIGNATURES = {
     "nvllm_b200_paged_decode_q8_workspace_bytes": (_sz, [_i32] * 3),
     "nvllm_b200_paged_decode_q8": (_i32, [_vp] * 9 + [_sz] + [_i32] * 7 + [_f32, _vp]),
     "nvllm_b200_decode_step_q8": (_i32, [_vp] * 12 + [_sz] + [_i32] * 7 + [_f32, _i32, _vp]),
+    "nvllm_b200_paged_prefill_q8_workspace_bytes": (_sz, [_i64] + [_i32] * 4),
     "nvllm_b200_paged_prefill_q8": (_i32, [_vp] * 11 + [_sz, _i64] + [_i32] * 8 + [_f32, _vp]),
     "nvllm_b200_copy_pages": (_i32, [_vp] * 3 + [_i32] + [_vp] * 3 + [_i32, _i64, _i32, _vp, _i64, _vp]),
 }

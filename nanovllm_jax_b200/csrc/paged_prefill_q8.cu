@@ -84,12 +84,18 @@ struct Whole : Params {
 struct Split : SplitParams {
     Source in;
 };
+struct Tail : TailParams {
+    Source in;
+};
+struct Work : Item {
+    int part;  // of a run: the place of its results
+};
 
 struct Shared {
     float q_factor[2][2][kTileQ];  // [item parity][Q tile][row]: what a row was divided by
     float4 scale[kInfos];          // of a tile: K scales of the first and second half, log2 of the V scales
     int token[kInfos];             // its first slot
-    Item items[kItemRing];         // the items of this CTA, written ahead by warp 3
+    Work items[kItemRing];         // the items of this CTA, written ahead by warp 3
     uint64_t item_full[kItemRing], item_empty[kItemRing];
     uint64_t q_full, q_empty;
     uint64_t factor_full[2];       // of the item parity: the softmax may come to an item when Q of the next one is there already
@@ -114,7 +120,7 @@ __device__ __forceinline__ bool wait_or_abort(Shared* sh, uint64_t* bar, uint32_
     return false;
 }
 
-__device__ __forceinline__ bool next_item(Shared* sh, uint32_t k, Item& it) {
+__device__ __forceinline__ bool next_item(Shared* sh, uint32_t k, Work& it) {
     const uint32_t slot = k % kItemRing;
     if (!wait_or_abort(sh, &sh->item_full[slot], (k / kItemRing) & 1u)) return false;
     it = sh->items[slot];
@@ -311,7 +317,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         if (lane == 0) {
             uint32_t t = 0, i = 0;  // tiles, items
             bool ok = true;
-            Item it = {};
+            Work it = {};
             int token = 0;
             float4 scale;
             float least = 0.f;  // log2 of the smallest V scale that counts
@@ -358,17 +364,28 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         // ============================== item records ================================
         if (lane == 0) {
             const List list = list_of(p);
-            const int total = tmem != 0xFFFFFFFFu ? items_of(p, list) : 0;
+            Cut cut = {items_of(static_cast<const Params&>(p), list), 1};
+            int total = cut.whole;
+            if constexpr (!std::is_same<P, Whole>::value) {
+                cut = cut_of(p, list);
+                total = cut.whole + (total - cut.whole) * cut.splits;
+            }
+            if (tmem == 0xFFFFFFFFu) total = 0;
             uint32_t k = 0;
             int idx = blockIdx.x;
             while (true) {
                 const uint32_t slot = k % kItemRing;
                 if (!wait_or_abort(sh, &sh->item_empty[slot], ((k / kItemRing) & 1u) ^ 1u)) break;
-                Item it;
+                Work it;
                 do {
                     if (k > 0 || idx != (int)blockIdx.x) idx = claim_item(p);
                     it.n_kv = -1;
-                    if (idx < total) it = load_item(p, list, idx);
+                    if (idx < total) {
+                        const int run = idx - cut.whole, c = run < 0 ? 0 : run % cut.splits;
+                        static_cast<Item&>(it) = load_item(static_cast<const Params&>(p), list, run < 0 ? idx : cut.whole + run / cut.splits);
+                        it.part = run;
+                        if (run >= 0) take_run(p, it, c, cut.splits);
+                    }
                     if (it.n_kv == 0) idx = total;  // nothing to do there: claim another one
                 } while (it.n_kv == 0);
                 sh->items[slot] = it;
@@ -397,7 +414,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             bool ok = true;
             auto k_full = [&](uint32_t t) { return wait_or_abort(sh, &sh->k_full[t % kSlots], (t / kSlots) & 1u); };
             auto v_full = [&](uint32_t t) { return wait_or_abort(sh, &sh->v_full[t % kVSlots], (t / kVSlots) & 1u); };
-            Item it;
+            Work it;
             while (ok && next_item(sh, i, it)) {
                 mbar_arrive(&sh->item_empty[i % kItemRing]);
                 const int n_x = x == 0 ? it.n_a : it.n_b, keys = keys_of(p, it, x, n_x), steps = n_x > 0 ? steps_of(keys) : 0;
@@ -469,7 +486,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         uint32_t kt = 0;  // K/V tiles of the items before this one
         uint32_t used = 0;  // of them, those in which this Q tile was active
         bool ok = true;
-        Item it;
+        Work it;
         for (uint32_t k = 0; ok && next_item(sh, k, it); ++k) {
             const int n_x = x == 0 ? it.n_a : it.n_b;
             const uint32_t kt0 = kt, g0 = g;
@@ -531,9 +548,9 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             tc_fence_after();
             ++used;
             const float in_units = fast_exp2(unit);
-            if constexpr (std::is_same<P, Split>::value) {
+            if constexpr (!std::is_same<P, Whole>::value) {
                 if (it.kv0 >= 0) {  // a run of a split item: its O, maximum and sum as they are
-                    float* part = p.partials + ((size_t)blockIdx.x * 2 + x) * kPartialFloats;
+                    float* part = p.partials + ((size_t)it.part * 2 + x) * kPartialFloats;
                     if (!dead) {
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {
@@ -602,7 +619,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
         const int w = warp - 12, r4 = lane >> 3, part = lane & 7;  // four rows of 128 bytes (16 per lane) at a time
         uint32_t t = 0;
         bool ok = true;
-        Item it;
+        Work it;
         for (uint32_t k = 0; ok && next_item(sh, k, it); ++k) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh->item_empty[k % kItemRing]);
@@ -717,7 +734,7 @@ static int ensure_attr() {
     NVLLM_CUDA_OK(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lock(mu);
     if (dev >= 0 && dev < 64 && !done[dev]) {
-        for (const void* f : {(const void*)paged_prefill_q8_kernel<Whole>, (const void*)paged_prefill_q8_kernel<Split>}) {
+        for (const void* f : {(const void*)paged_prefill_q8_kernel<Whole>, (const void*)paged_prefill_q8_kernel<Split>, (const void*)paged_prefill_q8_kernel<Tail>}) {
             cudaFuncAttributes a;
             NVLLM_CUDA_OK(cudaFuncGetAttributes(&a, f));
             if (a.numRegs != 128) return fail(NVLLM_B200_ECUDA, "paged_prefill_q8: built with %d registers, not the 128 it shares out", a.numRegs);
@@ -745,7 +762,7 @@ static int make_byte_map(CUtensorMap* map, const void* base, int heads, int64_t 
 }  // namespace prefill_q8
 
 namespace prefill {
-int launch_bytes(const Params& p, const SplitParams* split, const Bytes& in, const void* q, const void* k, const void* v, int64_t slots,
+int launch_bytes(const Params& p, const SplitParams* split, const TailParams* tail, const Bytes& in, const void* q, const void* k, const void* v, int64_t slots,
                  int KVH, cudaLaunchConfig_t cfg) {
     using namespace prefill_q8;
     int rc = ensure_attr();
@@ -760,6 +777,11 @@ int launch_bytes(const Params& p, const SplitParams* split, const Bytes& in, con
         static_cast<SplitParams&>(s) = *split;
         s.in = src;
         NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_prefill_q8_kernel<Split>, tm_k, s));
+    } else if (tail) {
+        Tail s;
+        static_cast<TailParams&>(s) = *tail;
+        s.in = src;
+        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_prefill_q8_kernel<Tail>, tm_k, s));
     } else {
         Whole s;
         static_cast<Params&>(s) = p;

@@ -41,6 +41,7 @@ struct Api {
     decltype(&nvllm_b200_paged_decode_q8_workspace_bytes) decode_q8_workspace_bytes;
     decltype(&nvllm_b200_paged_decode_q8) paged_decode_q8;
     decltype(&nvllm_b200_decode_step_q8) decode_step_q8;
+    decltype(&nvllm_b200_paged_prefill_q8_workspace_bytes) prefill_q8_workspace_bytes;
     decltype(&nvllm_b200_paged_prefill_q8) paged_prefill_q8;
     decltype(&nvllm_b200_copy_pages) copy_pages;
 } api = {};
@@ -786,7 +787,7 @@ PyObject* paged_prefill_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor out = output_like(a[11], q);
         same_device(q, {&out});
         zero_uncovered(host, b, out, t);
-        const at::Tensor ws = site.scratch(std::max<size_t>(api.prefill_workspace_bytes(t, b, h, c.kvh, c.d), 256));
+        const at::Tensor ws = site.scratch(std::max<size_t>(api.prefill_q8_workspace_bytes(t, b, h, c.kvh, c.d), 256));
         call([&] {
             return api.paged_prefill_q8(ptr(q), ptr(c.k), ptr(c.v), fptr(c.k_scale), fptr(c.v_scale), iptr(cu), iptr(cu_k), iptr(bt),
                                         host.data, mptr(out), mptr(ws), ws.nbytes(), t, b, max_seqlen_q, h, c.kvh, c.d, c.nb, c.block,
@@ -926,6 +927,7 @@ PyObject* bind(PyObject*, PyObject* args) {
         {"nvllm_b200_paged_decode_q8_workspace_bytes", (void**)&api.decode_q8_workspace_bytes},
         {"nvllm_b200_paged_decode_q8", (void**)&api.paged_decode_q8},
         {"nvllm_b200_decode_step_q8", (void**)&api.decode_step_q8},
+        {"nvllm_b200_paged_prefill_q8_workspace_bytes", (void**)&api.prefill_q8_workspace_bytes},
         {"nvllm_b200_paged_prefill_q8", (void**)&api.paged_prefill_q8},
         {"nvllm_b200_copy_pages", (void**)&api.copy_pages},
     };

@@ -113,7 +113,7 @@ constexpr int kPlanThreads = 1024;
 __global__ void __launch_bounds__(kPlanThreads) prefill_plan_kernel(const int32_t* __restrict__ cu_seqlens,
                                                                     const int32_t* __restrict__ cu_k, int paged, int B,
                                                                     int4* __restrict__ items, int capacity, int span,
-                                                                    int per_pair, int KVH, int ctas, int behind_store) {
+                                                                    int per_pair, int KVH, int ctas, int behind_store, int ordered) {
     // A token block's level is the number of K/V tiles in front of its last one (level_of).
     __shared__ int hist[kMaxLevels];
     __shared__ int base[kMaxLevels];
@@ -209,6 +209,34 @@ __global__ void __launch_bounds__(kPlanThreads) prefill_plan_kernel(const int32_
                 items[2 + 2 * slot] = make_int4(k_at[b], len_k, 0, 0);
             }
         }
+    }
+    if (ordered) {  // pairs of a level by sequence and token: which items are cut, and so the bits, depend on where they stand
+        __syncthreads();
+        const int n = items[0].x, i = threadIdx.x;
+        const bool mine = n <= kPlanThreads && i < n;
+        int4 q, k;
+        int to = i;
+        if (mine) {
+            q = items[1 + 2 * i], k = items[2 + 2 * i];
+            auto before = [&](int j, bool& same) {
+                const int4 qj = items[1 + 2 * j];
+                same = level_of(qj.y, items[2 + 2 * j].y, qj.z / span, span) == level_of(q.y, k.y, q.z / span, span);
+                return qj.w < q.w || (qj.w == q.w && qj.z < q.z);
+            };
+            bool same = true;
+            for (int j = i - 1; j >= 0; --j) {
+                const bool less = before(j, same);
+                if (!same) break;
+                to -= less ? 0 : 1;
+            }
+            for (int j = i + 1; j < n; ++j) {
+                const bool less = before(j, same);
+                if (!same) break;
+                to += less ? 1 : 0;
+            }
+        }
+        __syncthreads();
+        if (mine) items[1 + 2 * to] = q, items[2 + 2 * to] = k;
     }
     if (behind_store) {
         griddep_wait();
@@ -857,17 +885,19 @@ varlen_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_con
 // time, the ones that are not there included (a loop over the runs, unrolled by four, took the remainder one by one).
 constexpr int kCombineThreads = 128;
 constexpr int kCombineBatch = 8;
-__global__ void __launch_bounds__(kCombineThreads) prefill_combine_kernel(const __grid_constant__ SplitParams p) {
+template <class P>
+__global__ void __launch_bounds__(kCombineThreads) prefill_combine_kernel(const __grid_constant__ P p) {
     griddep_wait();
     const int e = blockIdx.x, x = blockIdx.y, row = blockIdx.z * 8 + (threadIdx.x >> 4), c8 = (threadIdx.x & 15) * 8;
     const List list = list_of(p);
-    if (e >= items_of(static_cast<const Params&>(p), list) || splits_of(p, list.pairs) == 1) return;
-    const Item it = load_item(static_cast<const Params&>(p), list, e);
-    const int runs = runs_of(p, p.splits, it.n_a, it.prefix, it.len_k);
+    const Cut cut = cut_of(p, list);
+    if (cut.whole + e >= items_of(static_cast<const Params&>(p), list) || cut.splits == 1) return;
+    const Item it = load_item(static_cast<const Params&>(p), list, cut.whole + e);
+    const int runs = runs_of(p, cut.splits, it.n_a, it.prefix, it.len_k);
     const int tok = row / p.pack.heads, q_pos = it.q0 + x * p.pack.dq + tok;
     if ((x == 0 ? it.n_a : it.n_b) == 0 || runs == 1 || tok >= p.pack.tokens || q_pos >= it.len) return;
     const int head = it.head + x * p.pack.dh + row - tok * p.pack.heads;
-    const float* part = p.partials + ((size_t)e * p.splits * 2 + x) * kPartialFloats;
+    const float* part = p.partials + ((size_t)e * cut.splits * 2 + x) * kPartialFloats;
     constexpr size_t kNext = 2 * kPartialFloats;
     float mv[kMaxSplits], m = -INFINITY;
 #pragma unroll
@@ -1074,6 +1104,8 @@ static int launch(const char* who, const void* q, const void* k, const void* v, 
         }
     }
 
+    const bool tail = bytes && splits == 1 && ((uintptr_t)workspace & 255) == 0 && tail_worth(pairs * p.per_pair, max_tiles, sms) &&
+                      workspace_bytes >= list_bytes(T, B, pack.span) + kTailSlots * partials_bytes(sms);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1087,7 +1119,7 @@ static int launch(const char* who, const void* q, const void* k, const void* v, 
         cfg.blockDim = dim3(kPlanThreads);
         NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, prefill_plan_kernel, cu_seqlens_q, cu_seqlens_k, block_tables ? 1 : 0, B,
                                          (int4*)workspace, (int)item_capacity(T, B, pack.span), pack.span, p.per_pair, KVH, ctas,
-                                         scatter && pdl_enabled() ? 1 : 0));
+                                         scatter && pdl_enabled() ? 1 : 0, tail ? 1 : 0));
     }
     cfg.gridDim = dim3((unsigned)ctas);
     cfg.blockDim = dim3(kThreads);
@@ -1100,17 +1132,27 @@ static int launch(const char* who, const void* q, const void* k, const void* v, 
         sp.ctas = (int)(pairs * p.per_pair * splits);
         cfg.gridDim = dim3((unsigned)sp.ctas);
         if (bytes) {
-            if ((rc = launch_bytes(p, &sp, *bytes, q, k, v, kv_tokens, KVH, cfg))) return rc;
+            if ((rc = launch_bytes(p, &sp, nullptr, *bytes, q, k, v, kv_tokens, KVH, cfg))) return rc;
         } else {
             NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<SplitParams>, tm_q, tm_k, tm_v, sp));
         }
         cfg.gridDim = dim3((unsigned)(pairs * p.per_pair), 2, kTileQ / 8);
         cfg.blockDim = dim3(kCombineThreads);
         cfg.dynamicSmemBytes = 0;
-        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, prefill_combine_kernel, sp));
-    } else if (bytes)
-        return launch_bytes(p, nullptr, *bytes, q, k, v, kv_tokens, KVH, cfg);
-    else if (brief)
+        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, prefill_combine_kernel<SplitParams>, sp));
+    } else if (bytes) {
+        if (!tail) return launch_bytes(p, nullptr, nullptr, *bytes, q, k, v, kv_tokens, KVH, cfg);
+        TailParams tp;
+        static_cast<Params&>(tp) = p;
+        tp.partials = (float*)((uint8_t*)workspace + list_bytes(T, B, pack.span));
+        tp.ctas = sms;
+        cfg.gridDim = dim3((unsigned)sms);
+        if ((rc = launch_bytes(p, nullptr, &tp, *bytes, q, k, v, kv_tokens, KVH, cfg))) return rc;
+        cfg.gridDim = dim3((unsigned)sms, 2, kTileQ / 8);
+        cfg.blockDim = dim3(kCombineThreads);
+        cfg.dynamicSmemBytes = 0;
+        NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, prefill_combine_kernel<TailParams>, tp));
+    } else if (brief)
         NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<ShortParams>, tm_q, tm_k, tm_v, p));
     else
         NVLLM_CUDA_OK(cudaLaunchKernelEx(&cfg, varlen_prefill_kernel<Params>, tm_q, tm_k, tm_v, (const Params&)p));
@@ -1142,6 +1184,18 @@ extern "C" size_t nvllm_b200_varlen_prefill_workspace_bytes(int64_t T, int B, in
     const int64_t blocks = std::max<int64_t>((T + pack.span - 1) / pack.span, B), per_pair = (int64_t)KVH * pack.per_kv;
     if (2 * blocks * per_pair <= sm_count())
         n = list_bytes(T, B, make_pack(H / KVH, true).span) + partials_bytes(sm_count());
+    return n;
+}
+
+extern "C" size_t nvllm_b200_paged_prefill_q8_workspace_bytes(int64_t T, int B, int H, int KVH, int D) {
+    using namespace nvllm;
+    using namespace nvllm::prefill;
+    size_t n = nvllm_b200_varlen_prefill_workspace_bytes(T, B, H, KVH, D);
+    if (T < 0 || B < 0 || H <= 0 || KVH <= 0 || H % KVH != 0) return n;
+    // and for the runs of a last round
+    const Pack pack = make_pack(H / KVH);
+    const int64_t blocks = std::max<int64_t>((T + pack.span - 1) / pack.span, B), per_pair = (int64_t)KVH * pack.per_kv;
+    if (blocks * per_pair <= (int64_t)kTailRounds * sm_count()) n = std::max(n, list_bytes(T, B, pack.span) + kTailSlots * partials_bytes(sm_count()));
     return n;
 }
 

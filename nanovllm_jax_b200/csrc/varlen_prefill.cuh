@@ -109,6 +109,12 @@ __device__ __forceinline__ int items_of(const SplitParams& p, const List& l) {
     return l.pairs * p.per_pair * splits_of(p, l.pairs);
 }
 
+// Items of which the last ones are cut: `whole` in front stay as they are, of those behind every one is `splits` runs.
+struct Cut {
+    int whole, splits;
+};
+__device__ __forceinline__ Cut cut_of(const SplitParams& p, const List& l) { return Cut{0, splits_of(p, l.pairs)}; }
+
 // ------------------------------------------------------------------------------------------
 // tcgen05 wrappers
 // ------------------------------------------------------------------------------------------
@@ -292,18 +298,14 @@ __device__ __forceinline__ Item load_item(const Params& p, const List& l, int id
     const int pair = idx / per;
     return make_item(p, record_of(p, pair), first + idx - pair * per);
 }
-__device__ __forceinline__ Item load_item(const SplitParams& p, const List& l, int idx) {
-    const int splits = splits_of(p, l.pairs), c = idx % splits;
-    Item it = load_item(static_cast<const Params&>(p), l, idx / splits);
+// Run c of an item that is cut into up to `splits`; one with nothing to do (n_kv = 0) where it has fewer.
+__device__ __forceinline__ void take_run(const Params& p, Item& it, int c, int splits) {
     const int runs = runs_of(p, splits, it.n_a, it.prefix, it.len_k);
-    if (runs == 1) {
-        if (c > 0) it.n_a = it.n_b = it.n_kv = 0;
-        return it;
-    }
     if (c >= runs) {
         it.n_a = it.n_b = it.n_kv = 0;
-        return it;
+        return;
     }
+    if (runs == 1) return;
     const int j0 = it.n_a * c / runs, j1 = c + 1 == runs ? it.n_kv : it.n_a * (c + 1) / runs;
     it.kv0 = j0;
     it.n_a = min(it.n_a, j1) - j0;
@@ -311,7 +313,42 @@ __device__ __forceinline__ Item load_item(const SplitParams& p, const List& l, i
     it.n_kv = j1 - j0;
     it.len_k -= j0 * kTileKV;
     it.prefix -= j0 * kTileKV;
+}
+__device__ __forceinline__ Item load_item(const SplitParams& p, const List& l, int idx) {
+    const int splits = splits_of(p, l.pairs), c = idx % splits;
+    Item it = load_item(static_cast<const Params&>(p), l, idx / splits);
+    take_run(p, it, c, splits);
     return it;
+}
+
+// A few rounds of items, each an SM's work for a long time: those of the last round, which leaves SMs idle, are cut into runs as well.  `ctas`:
+// the launch's, which claim the items in their order and then the runs.  (8-bit pages only: packed bf16 keys and bf16 keys in pages
+// are to give the same bits.)  Whole and cut, 32 / 8 heads: 1280 new tokens (160 items) behind 30 000 1058 and 665 us, behind 8000 310 and 216,
+// behind 2500 130 and 120; 640 (80 items) behind 8000 158 and 142; 2560 (320) 479 and 432; 20 x 64 behind 3000 127 and 110.  Twice the room
+// for results lets 2048 (256) be cut, too: 345 instead of 335, for at the power cap what idle SMs leave makes the others faster.
+struct TailParams : Params {
+    float* partials;  // [kTailSlots * ctas][Q tile][kPartialFloats]
+    int ctas;
+};
+constexpr int kTailRounds = 3;  // there is a quarter to be gained at most behind more
+constexpr int kTailSlots = 2;
+constexpr int kTailRuns = 8;
+// In K/V tiles' time: what a run costs beside its own (start, first scores, its results to memory), and the launch that combines them.
+constexpr int kRunCost = 2, kCombineCost = 4;
+// Runs for each of n items (fewer than CTAs) of so many K/V tiles: the number that ends first, 1 where that is the items as they are.
+__host__ __device__ __forceinline__ int tail_runs(int n, int tiles, int ctas) {
+    int best = 1, least = tiles < 2 * kSplitTiles ? 0 : tiles;
+    for (int s = 2; s <= kTailRuns && n * s <= kTailSlots * ctas; ++s) {
+        const int t = (n * s + ctas - 1) / ctas * ((tiles + s - 1) / s + kRunCost) + kCombineCost;
+        if (t < least) least = t, best = s;
+    }
+    return best;
+}
+__device__ __forceinline__ Cut cut_of(const TailParams& p, const List& l) {
+    const int total = items_of(static_cast<const Params&>(p), l), whole = total / p.ctas * p.ctas, n = total - whole;
+    if (n == 0 || total > kTailRounds * p.ctas) return Cut{total, 1};
+    const int runs = tail_runs(n, load_item(static_cast<const Params&>(p), l, whole).n_kv, p.ctas);
+    return runs == 1 ? Cut{total, 1} : Cut{whole, runs};
 }
 
 // The output is marked as evicted first, so that it does not push keys and values out of the L2 (16 prompts of 128..4096 tokens, 32 / 8
@@ -340,13 +377,17 @@ inline bool lone_tiles(int64_t max_tiles, int splits, int lone_splits, int64_t l
     return (max_tiles + lone_splits - 1) / lone_splits <= (max_tiles + splits - 1) / splits + more;
 }
 inline size_t partials_bytes(int sms) { return (size_t)sms * 2 * kPartialFloats * 4; }
+// Whether `items` of up to max_tiles K/V tiles (bounds of what the device will find) leave a last round that is worth cutting.
+inline bool tail_worth(int64_t items, int64_t max_tiles, int sms) {
+    return 2 * items > sms && items <= (int64_t)kTailRounds * sms && items % sms && tail_runs((int)(items % sms), (int)max_tiles, sms) > 1;
+}
 
-// Keys and values in 8-bit pages: the main kernel is another one (paged_prefill_q8.cu).  `split`: for runs, or null.
+// Keys and values in 8-bit pages: the main kernel is another one (paged_prefill_q8.cu).  `split`, `tail`: for runs, or null.
 struct Bytes {
     const float *k_scale, *v_scale;
     int NB;
 };
-int launch_bytes(const Params& p, const SplitParams* split, const Bytes& in, const void* q, const void* k, const void* v, int64_t slots,
+int launch_bytes(const Params& p, const SplitParams* split, const TailParams* tail, const Bytes& in, const void* q, const void* k, const void* v, int64_t slots,
                  int KVH, cudaLaunchConfig_t cfg);
 
 }  // namespace prefill

@@ -245,3 +245,38 @@ def test_nan_query_of_a_split_sequence():
     q[2, 3] = 0
     out[2, 3] = clean[2, 3]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("h, kvh, new, pre", [
+    (8, 8, [1] * 10, [8000 - 64 * i for i in range(10)]),                # 80 items: one round, all of them in runs
+    (8, 8, [1, 2, 130, 300] * 5, [5000, 4100, 2000, 129] * 5),           # a round and a few items, of unlike length
+    (16, 2, [40] * 45, [1500 + 40 * (i % 20) for i in range(45)]),       # both tiles of the same keys; a round and most of another
+    (3, 1, [12000], [300])])                                             # a long prompt: three tokens' heads in turn over the tiles
+def test_last_round_in_runs(h, kvh, new, pre):
+    """More items than half the SMs, in few rounds, with many keys each: against attention over the dequantised cache and, where it is
+    quick, the 64-bit statement; the same bits when called again and when captured with other lengths."""
+    import torch
+    from nanovllm_jax_b200 import _lib, ops
+    rng = np.random.default_rng(h + len(new))
+    q, tables, cu, cu_k, cu_host, nb, lens = make(rng, new, pre, h, kvh, 256)
+    cache = random_cache(rng, nb, 256, kvh)
+    out = ops.paged_prefill_q8(q, *cache, tables, cu, cu_k, max(new), 0.0884, 256)
+    if sum(new) <= 20:
+        close(out, expect(q, cache, tables, new, lens, 0.0884, 256), q, 0.0884, key_size(cache))
+    wide = [(c.float() * s.repeat_interleave(64, 1)[..., None]).to(torch.bfloat16) for c, s in zip(cache[:2], cache[2:])]
+    want = ops.paged_prefill(q, *wide, tables, cu, cu_k, max(new), 0.0884, 256).float()
+    # as in test_against_the_bf16_kernel_over_the_same_values
+    assert ((out.float() - want).norm() / want.norm()) < 2.0 ** -8 * math.sqrt(2)
+    assert (out.float() - want).abs().max() < 2.0 ** -6 * wide[1].float().abs().max()
+    for _ in range(5):
+        assert torch.equal(out, ops.paged_prefill_q8(q, *cache, tables, cu, cu_k, max(new), 0.0884, 256))
+    # captured where every sequence has one new token, replayed with these: more items than the host could foresee, or fewer
+    one = torch.arange(len(new) + 1, dtype=torch.int32).cuda()
+    at, at_k, got = one.clone(), torch.cat([one[:1], (one[1:] * 0 + 2100).cumsum(0, dtype=torch.int32)]), torch.zeros_like(out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_prefill_q8(q, *cache, tables, at, at_k, max(new), 0.0884, 256, out=got)
+    at.copy_(cu), at_k.copy_(cu_k)
+    graph.replay()
+    assert ((got.float() - want).norm() / want.norm()) < 2.0 ** -8 * math.sqrt(2)
+    assert _lib.device_status() == 0
