@@ -392,8 +392,12 @@ int nvllm_b200_decode_step_q8(const void* q, const void* k, const void* v, void*
                               int KVH, int D, int NB, int block_size, int MB, float scale, int src_dtype, void* stream);
 
 /*
- * paged_prefill_q8: nvllm_b200_paged_prefill over an 8-bit cache (block_size a multiple of 128); the arguments they share, the
- * workspace and the device status bits mean the same.  The new tokens' rows must have been stored already.
+ * paged_prefill_q8: nvllm_b200_paged_prefill over an 8-bit cache (block_size a multiple of 128); the arguments they share and
+ * the device status bits mean the same.  The new tokens' rows must have been stored already.
+ *
+ *   workspace     >= nvllm_b200_paged_prefill_q8_workspace_bytes(T, B, H, KVH, D) bytes, 256-byte aligned (the size of
+ *                 nvllm_b200_varlen_prefill_workspace_bytes will do, but some calls take longer with it)
+ *
  * Math: scores in fp32 from the cache's own values and from q as the sum of two e4m3 numbers under a power of two per row (exact
  * for components above 2^-11 of the row's largest, to within 2^-18 of it for smaller ones); fp16 probabilities, which carry the V
  * scale, times the cache's own values in fp16 (exact) into fp32.  What a probability loses by underflow is relative to the row's
