@@ -646,7 +646,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             for (int x = 0; x < q_tiles; ++x) {
                 const int live = min(p.pack.tokens, it.len - (it.q0 + x * p.pack.dq));
                 const int groups = min(8, (live * p.pack.heads + 15) >> 4);  // of 16 rows, that hold live ones
-#pragma unroll 2
+#pragma unroll 1
                 for (int s = 0; s < groups; ++s) {
                     const int row = s * 16 + w * 4 + r4;
                     uint4* const at = reinterpret_cast<uint4*>(smem + x * kTileBytes + row * 128 + ((part ^ (row & 7)) << 4));
@@ -661,13 +661,8 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     for (int step = 1; step < 8; step <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
                     const q8::RowPower power(top);
                     uint32_t hi[4], lo[4];
-                    if (__any_sync(0xffffffffu, top >= 0x7f80u)) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) q8::split_row<true>(in[2 * c], in[2 * c + 1], power.down, hi[c], lo[c]);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) q8::split_row<false>(in[2 * c], in[2 * c + 1], power.down, hi[c], lo[c]);
-                    }
+                    for (int c = 0; c < 4; ++c) q8::split_row(in[2 * c], in[2 * c + 1], power.down, hi[c], lo[c]);
                     *at = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     *at_lo = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     if (part == 0) sh->q_factor[k & 1][x][row] = power.up;

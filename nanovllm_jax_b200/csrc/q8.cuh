@@ -47,24 +47,21 @@ __device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two_bytes) {
 }
 
 // A bf16 row as the sum of two e4m3 rows.  `top`: its largest magnitude's bits.  The row is multiplied by `down`, a power of two
-// that brings the largest magnitude to 224 < .. <= 448; `up` is its inverse.  A row of zeros stays as it is.
+// that brings the largest magnitude to 224 < .. <= 448; `up` is its inverse.  A row of zeros stays as it is; one with a NaN or an
+// infinity, whose softmax is NaN whatever the keys are, becomes NaN.
 struct RowPower {
     float down, up;
     __device__ __forceinline__ explicit RowPower(uint32_t top) {
         const uint32_t shift = (top & 0x7fu) <= 0x60u ? 8 : 7, e = min(max(top == 0 ? 127u + shift : top >> 7, 9u), 254u);
-        down = __uint_as_float((254u + shift - e) << 23);
+        down = __uint_as_float(top < 0x7f80u ? (254u + shift - e) << 23 : 0x7fffffffu);
         up = __uint_as_float((e - shift) << 23);
     }
 };
 // Four elements (two words of bf16) -> upper and lower parts, a byte each: hi = e4m3(x), lo = e4m3(x - hi).  bf16 has eight
-// significant bits and e4m3 four, so the sum is exact where lo is no subnormal.  What is not finite becomes NaN (CAREFUL: there may be
-// such).
-template <bool CAREFUL>
+// significant bits and e4m3 four, so the sum is exact where lo is no subnormal.
 __device__ __forceinline__ void split_row(uint32_t w0, uint32_t w1, float down, uint32_t& hi, uint32_t& lo) {
-    float f[4] = {__uint_as_float(w0 << 16) * down, __uint_as_float(w0 & 0xffff0000u) * down, __uint_as_float(w1 << 16) * down,
+    const float f[4] = {__uint_as_float(w0 << 16) * down, __uint_as_float(w0 & 0xffff0000u) * down, __uint_as_float(w1 << 16) * down,
                   __uint_as_float(w1 & 0xffff0000u) * down};
-#pragma unroll
-    for (int i = 0; CAREFUL && i < 4; ++i) f[i] = fabsf(f[i]) < INFINITY ? f[i] : __uint_as_float(0x7fffffffu);
     const uint32_t h0 = to_e4m3x2(f[0], f[1]), h1 = to_e4m3x2(f[2], f[3]);
     const float2 g0 = e4m3x2_to_float2(h0), g1 = e4m3x2_to_float2(h1);
     hi = h0 | h1 << 16;
