@@ -4,7 +4,7 @@
 // The scale that the store chooses is a power of two, 2^k with the smallest k for which the largest finite magnitude of the
 // block is at most 448 * 2^k.  e4m3 is a floating format, so a scale's fraction would buy no precision; a power of two makes
 // a later change of the scale exact except where a value becomes subnormal, and value * scale a bf16 number (four
-// significant bits), so attention over the 8-bit cache can be held bit for bit against attention over the same cache in bf16.
+// significant bits): the same cache in bf16 holds the same keys and values.
 #pragma once
 
 #include "common.cuh"

@@ -1192,10 +1192,11 @@ extern "C" size_t nvllm_b200_paged_prefill_q8_workspace_bytes(int64_t T, int B, 
     using namespace nvllm::prefill;
     size_t n = nvllm_b200_varlen_prefill_workspace_bytes(T, B, H, KVH, D);
     if (T < 0 || B < 0 || H <= 0 || KVH <= 0 || H % KVH != 0) return n;
-    // and for the runs of a last round
+    // and for the runs of a last round, where there may be more items than half the SMs (up to twice as many as blocks)
     const Pack pack = make_pack(H / KVH);
     const int64_t blocks = std::max<int64_t>((T + pack.span - 1) / pack.span, B), per_pair = (int64_t)KVH * pack.per_kv;
-    if (blocks * per_pair <= (int64_t)kTailRounds * sm_count()) n = std::max(n, list_bytes(T, B, pack.span) + kTailSlots * partials_bytes(sm_count()));
+    if (4 * blocks * per_pair > sm_count() && blocks * per_pair <= (int64_t)kTailRounds * sm_count())
+        n = std::max(n, list_bytes(T, B, pack.span) + kTailSlots * partials_bytes(sm_count()));
     return n;
 }
 
