@@ -560,7 +560,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
 #pragma unroll
                             for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * in_units);
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
+                            for (int i = 0; i < 8 && tok < live; ++i)
                                 *reinterpret_cast<uint4*>(part + row * kD + c * 32 + i * 4) =
                                     make_uint4(ov[4 * i], ov[4 * i + 1], ov[4 * i + 2], ov[4 * i + 3]);
                         }
@@ -630,8 +630,9 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             const int q_tiles = it.n_b > 0 ? 2 : 1;
             for (int x = 0; x < q_tiles; ++x) {
                 const int q_pos = it.q0 + x * p.pack.dq, live = min(p.pack.tokens, it.len - q_pos);
-#pragma unroll
-                for (int s = 0; s < 8; ++s) {
+                const int groups = min(8, (live * p.pack.heads + 15) >> 4);  // of 16 rows, that hold live ones
+#pragma unroll 4
+                for (int s = 0; s < groups; ++s) {
                     const int row = s * 16 + w * 4 + r4, tok = row / p.pack.heads;
                     const int head = it.head + x * p.pack.dh + row - tok * p.pack.heads;
                     const bool in = tok < live;
@@ -645,7 +646,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             asm volatile("cp.async.wait_all;" ::: "memory");
             for (int x = 0; x < q_tiles; ++x) {
                 const int live = min(p.pack.tokens, it.len - (it.q0 + x * p.pack.dq));
-                const int groups = min(8, (live * p.pack.heads + 15) >> 4);  // of 16 rows, that hold live ones
+                const int groups = min(8, (live * p.pack.heads + 15) >> 4);
 #pragma unroll 1
                 for (int s = 0; s < groups; ++s) {
                     const int row = s * 16 + w * 4 + r4;
