@@ -258,11 +258,20 @@ struct Site {
     const at::Tensor& scratch(size_t nbytes) const { return workspace(device, stream, nbytes); }
 };
 
+// The launches of a call go to its stream one behind the other: another thread's call on the same stream, which shares the scratch
+// buffer, must not come between them.
+std::mutex& issue_mutex() {
+    static auto* m = new std::mutex();
+    return *m;
+}
 template <class F>
 void call(F&& f) {
     int rc;
     Py_BEGIN_ALLOW_THREADS;
-    rc = f();
+    {
+        const std::lock_guard<std::mutex> lock(issue_mutex());
+        rc = f();
+    }
     Py_END_ALLOW_THREADS;
     if (rc != NVLLM_B200_OK) {
         PyObject* r = PyObject_CallFunction(check_fn, "i", rc);

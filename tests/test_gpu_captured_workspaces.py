@@ -1,5 +1,5 @@
-"""Scratch buffers of captured graphs: two graphs that were captured on one stream are replayed side by side on two others, beside
-eager calls on the capture's own stream."""
+"""Scratch buffers: two graphs that were captured on one stream are replayed side by side on two others, beside eager calls on the
+capture's own stream; two threads call on one stream."""
 import gc
 import time
 
@@ -96,3 +96,34 @@ def test_buffers_go_with_their_graph():
             call()
         held.append(torch.cuda.memory_allocated())
     assert max(held) <= held[0], held
+
+
+def test_two_threads_on_one_stream():
+    import threading
+    import torch
+    from nanovllm_jax_b200 import _lib
+    jobs = [work(s) for s in (7, 8)]
+    want = []
+    for call, written in jobs:
+        call()
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in written])
+    wrong = []
+
+    def loop(i):
+        call, written = jobs[i]
+        try:
+            for _ in range(60):
+                call()
+            torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(written, want[i])):
+                wrong.append(i)
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    threads = [threading.Thread(target=loop, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and _lib.device_status() == 0
