@@ -12,9 +12,10 @@
 //    (CTAs that look through all slots themselves, while their rows are on their way, are no better in between: 48 prompts of
 //    5..300 tokens, fp32, 2 kv heads: 11.1 us, with the kernel in front 9.6.)
 //
-// Measured: 16 prompts of 128..4096 tokens, 8 kv heads, bf16: 42.3 us, 4.9 TB/s, 0.76 of a plain copy's rate (loads in flight and issue
-// slots, 0.6 of which are taken, share the bound; asking for the window's rows before its slots are known: 43.6; 128 tokens a CTA:
-// 44.9); 64 appended rows 4 to 5 us.
+// Measured: 16 prompts of 128..4096 tokens, 8 kv heads, bf16: 42.3 us, 4.9 TB/s, 0.76 of a plain copy's rate (the chain slots -> rows
+// -> scale -> stores of four CTAs per SM: without the arithmetic it takes as long, without the stores 35 us; the window's rows asked for
+// before its slots are known: 43.6; 128 tokens a CTA: 44.9; CTAs that stay and have the next window's slots at hand: 48.7, for
+// they spill); 64 appended rows 4 to 5 us.
 #include "store_kvcache_q8.cuh"
 
 #include <algorithm>

@@ -85,6 +85,15 @@ def test_many_random_pairs(n):
         check(c, rng.integers(-20, 2020, n), rng.integers(-20, 2020, n), 64, tokens=rng.integers(0, 65, n), tables=rng.integers(-1, 2000, (3, 50)))
 
 
+def test_a_tensor_twice_and_views():
+    """The same tensor, and another shape of it, in one list: every copy of a page writes what the others write."""
+    rng = np.random.default_rng(4)
+    c = caches(rng, 9, 64, 2, "bf16", 1)
+    assert not check([c[0], c[1], c[0], c[0].view(9, 64, 256)], [0, 1, 7], [2, 3, 8], 64, tokens=[64, 5, 0])
+    assert not check([c[0].view(9, 32, 512), c[0]], [0], [5], 64)
+    assert np.array_equal(host(c[0][5]), host(c[0][0]))  # bits: there are NaNs among them
+
+
 def test_captured_and_replayed():
     import torch
     from nanovllm_jax_b200 import ops
