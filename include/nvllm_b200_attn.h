@@ -383,7 +383,7 @@ int nvllm_b200_paged_decode_q8(const void* q, const void* k_cache, const void* v
 
 /*
  * decode_step_q8: nvllm_b200_store_kvcache_q8 (T = B) followed by nvllm_b200_paged_decode_q8, as one C call and two launches
- * (four beyond 1024 sequences): a decode step of the attention layer (layers/attention.py:436-480) over an 8-bit cache.
+ * (four beyond 4096 sequences): a decode step of the attention layer (layers/attention.py:436-480) over an 8-bit cache.
  * Same workspace size as nvllm_b200_paged_decode_q8.
  */
 int nvllm_b200_decode_step_q8(const void* q, const void* k, const void* v, void* k_cache, void* v_cache, float* k_scale,

@@ -519,7 +519,7 @@ paged_decode_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_co
     }
 }
 
-// In front of the kernel above: clears the tickets and, in a decode step of up to kScanTokens sequences, stores the step's rows
+// In front of the kernel above: clears the tickets and, in a decode step of up to kScanStep sequences, stores the step's rows
 // (blocks [0, store_blocks): a token and kv head each).
 template <typename SrcT>
 __global__ void __launch_bounds__(q8::kStoreThreads)
@@ -551,7 +551,7 @@ static int ensure_smem_attr() {
 }
 
 static size_t workspace_bytes_for(int B, int H, int KVH, bool step) {
-    return ticket_bytes(B, KVH) + partial_bytes(grid(), H / KVH) + (step && B > q8::kScanTokens ? q8::store_workspace_bytes(B) : 0) + 256;
+    return ticket_bytes(B, KVH) + partial_bytes(grid(), H / KVH) + (step && B > q8::kScanStep ? q8::store_workspace_bytes(B) : 0) + 256;
 }
 
 // `step`: the store of a decode step (T = B), or null.
@@ -607,7 +607,7 @@ static int run(const char* who, const DecodeArgs& a, const float* k_scale, const
 
     const int num_tickets = a.B * a.KVH;
     const int clear_blocks = (num_tickets + q8::kStoreThreads - 1) / q8::kStoreThreads;
-    const bool inside = step && a.B <= q8::kScanTokens;
+    const bool inside = step && a.B <= q8::kScanStep;
     if (step && !inside &&
         (rc = q8::launch_store(who, *step, src_dtype, ws + ticket_bytes(a.B, a.KVH) + partial_bytes(grid(), p.G),
                                q8::store_workspace_bytes(a.B), cfg.stream)))

@@ -44,7 +44,7 @@ def test_decode(lib):
     need = lib.nvllm_b200_paged_decode_q8_workspace_bytes(4, 8, 2)
     assert decode(lib, ws=None) == decode(lib, wsn=need // 2) == decode(lib, ws=P + 16) == _lib.EWORKSPACE
     assert decode(lib, b=0, q=None) == _lib.OK
-    assert lib.nvllm_b200_paged_decode_q8_workspace_bytes(2000, 8, 2) > need + lib.nvllm_b200_store_kvcache_q8_workspace_bytes(2000)
+    assert lib.nvllm_b200_paged_decode_q8_workspace_bytes(5000, 8, 2) > need + lib.nvllm_b200_store_kvcache_q8_workspace_bytes(5000)
 
 
 def test_decode_step(lib):

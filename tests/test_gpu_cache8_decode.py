@@ -125,7 +125,7 @@ def test_rows_behind_the_context_may_hold_anything():
 
 
 @pytest.mark.parametrize("f32", (False, True))
-@pytest.mark.parametrize("batch, block", [(1, 64), (5, 128), (40, 256), (300, 64), (1100, 64)])
+@pytest.mark.parametrize("batch, block", [(1, 64), (5, 128), (40, 256), (300, 64), (1100, 64), (4200, 64)])
 def test_step_is_store_then_decode(batch, block, f32):
     import torch
     from nanovllm_jax_b200 import ops

@@ -19,7 +19,7 @@ def check(k, v, cache, slots, what=""):
     for x, rows in enumerate((k, v)):
         flat, grid = before[x].reshape(-1, kvh, 128), before[2 + x].reshape(-1, kvh)
         values, scales = cache8.store(rows.double().cpu().numpy(), flat, grid, slots.cpu().numpy())
-        assert np.array_equal(cache[2 + x].double().cpu().numpy().reshape(scales.shape), scales), f"{what}: scales {'kv'[x]}"
+        assert np.array_equal(cache[2 + x].double().cpu().numpy().reshape(scales.shape), scales, equal_nan=True), f"{what}: scales {'kv'[x]}"
         got = values_of(cache[x]).reshape(values.shape)
         assert np.array_equal(got, values, equal_nan=True), f"{what}: {'kv'[x]}, slots {np.unique(np.nonzero(~((got == values) | (np.isnan(got) & np.isnan(values))))[0])[:8]}"
 
@@ -64,6 +64,27 @@ def test_appended_rows_let_the_scale_grow(t, kvh, block):
     slots = (grains * 64 + rng.integers(0, 64, t)).astype(np.int32)
     k, v = rows(rng, t, kvh, torch.bfloat16, spread=9)
     check(k, v, random_cache(rng, nb, block, kvh), torch.from_numpy(slots).cuda())
+
+
+@pytest.mark.parametrize("f32", (False, True))
+@pytest.mark.parametrize("t, kvh", [(128, 8), (129, 8), (600, 8), (1024, 3), (400, 5)])
+def test_rows_alone_in_their_blocks(t, kvh, f32):
+    """A decode step's rows, few and many: first slots of blocks and later ones, scales that are none, values that are not finite, and among
+    them a few blocks that other rows of the call go to as well."""
+    import torch
+    rng = np.random.default_rng(t + kvh)
+    block, nb = 128, t + 1
+    grains = rng.permutation(2 * nb)[:t]
+    grains[t // 2], grains[t - 1] = grains[3], grains[3]  # one block three times, far apart
+    slots = (grains * 64 + np.where(rng.random(t) < 0.2, 0, rng.integers(0, 64, t))).astype(np.int32)
+    slots[5] = -1
+    k, v = rows(rng, t, kvh, torch.float32 if f32 else torch.bfloat16, spread=9)
+    k[7, 0, 3], k[8, 1], v[9, :, 100], v[10] = float("inf"), float("nan"), -float("inf"), 0
+    cache = random_cache(rng, nb, block, kvh)
+    cache[2].view(-1)[::7] = 0
+    cache[3].view(-1)[::5] = float("nan")
+    cache[3].view(-1)[1::5] = -1
+    check(k, v, cache, torch.from_numpy(slots).cuda())
 
 
 @pytest.mark.parametrize("t", (7, 700, 1024, 1030, 4000))
