@@ -15,7 +15,8 @@
 // Measured: 16 prompts of 128..4096 tokens, 8 kv heads, bf16: 42.3 us, 4.9 TB/s, 0.76 of a plain copy's rate (the chain slots -> rows
 // -> scale -> stores of four CTAs per SM: without the arithmetic it takes as long, without the stores 35 us; the window's rows asked for
 // before its slots are known: 43.6; 128 tokens a CTA: 44.9; CTAs that stay and have the next window's slots at hand: 48.7, for
-// they spill); 64 appended rows 4 to 5 us.
+// they spill); 64 appended rows 4 to 5 us.  More than 1024 appended rows go one after the other, 64 a CTA: 2000, 8 kv heads, 80 us; a warp
+// each in the same kernel 13, but the prompts then take 47 (a decode step has another way, see kScanStep).
 #include "store_kvcache_q8.cuh"
 
 #include <algorithm>
