@@ -403,6 +403,7 @@ int nvllm_b200_decode_step_q8(const void* q, const void* k, const void* v, void*
  * scale, times the cache's own values in fp16 (exact) into fp32.  What a probability loses by underflow is relative to the row's
  * largest one and to the largest V scale among the keys before it: at most 2^-32 of their product times 448; a V scale below 2^-64 of that
  * one counts as 2^-64 of it.
+ * A NaN in the cache (what a NaN or an infinity was stored as) reaches the rows that see its token, of K every dim, of V its own.
  */
 size_t nvllm_b200_paged_prefill_q8_workspace_bytes(int64_t T, int B, int H, int KVH, int D);
 int nvllm_b200_paged_prefill_q8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,

@@ -107,6 +107,7 @@ struct Shared {
     uint64_t s_full[2][2], p_full[2][2];  // [Q tile][step parity]
     uint64_t o_done[2][2];               // [Q tile][an item's last step but one (or only one), its last one]
     uint64_t o_empty[2];
+    uint32_t odd_values[2];              // of the item parity: 1 + the item of which V held NaN behind a row's limit (see add_nan)
     uint32_t tmem_base;
     volatile int abort_flag;
 };
@@ -257,6 +258,45 @@ __device__ __forceinline__ bool softmax_step(Shared* sh, const uint32_t t_s, con
     return true;
 }
 
+// K/V tiles in front of the first one of which the item's first row does not see every key.
+__device__ __forceinline__ int plain_tiles(const Item& it) { return (it.prefix + it.q0 + 1) / kTileKV; }
+
+// Whether a byte of w is NaN: its bit 7.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return (w & 0x7f7f7f7fu) + 0x01010101u; }
+
+// P is 0 for a key behind a row's limit, but 0 * NaN is NaN: a NaN there would reach rows that do not see it.  In the tiles that hold
+// such keys V has 0 in its place, and here O gets it back in the rows that do see it: every row reads the bytes again for itself, up to
+// its own limit.  Called by a warp of the softmax for its rows, of Q tile x and its token tok each.  Only what is not finite is stored
+// as NaN, so this is rare; a call, which costs the others nothing (in the loops that read O it made eight runs of four steps, 25.2 us,
+// half a microsecond longer).
+__device__ __noinline__ void add_nan(const Params& p, const Source& in, const Work& it, int x, int tok, uint32_t t_o) {
+    const int q_pos = it.q0 + x * p.pack.dq, tiles = x == 0 ? it.n_a : it.n_b;
+    const int seen = tok < min(p.pack.tokens, it.len - q_pos) ? it.prefix + q_pos + tok + 1 : 0;  // keys of the row
+#pragma unroll 1
+    for (int c = 0; c < 8; ++c) {  // 16 dims at a time
+        uint32_t odd[4] = {0u, 0u, 0u, 0u};
+        for (int j = plain_tiles(it); j < tiles; ++j) {
+            const int off = (max(it.kv0, 0) + j) * kTileKV;
+            const int page = __ldg(p.block_tables + (size_t)it.b * p.MB + min(off / p.block_size, p.MB - 1));
+            const int token = min(max(page, 0), in.NB - 1) * p.block_size + off % p.block_size;
+            const uint8_t* at = in.v + ((size_t)token * in.KVH + it.kvh) * kD + c * 16;
+            const int keys = min(kTileKV, seen - j * kTileKV);
+            for (int i = 0; i < keys; ++i, at += (size_t)in.KVH * kD) {
+                const uint4 w = __ldg(reinterpret_cast<const uint4*>(at));
+                odd[0] |= nan_bytes(w.x), odd[1] |= nan_bytes(w.y), odd[2] |= nan_bytes(w.z), odd[3] |= nan_bytes(w.w);
+            }
+        }
+        __syncwarp();
+        uint32_t ov[16];
+        tmem_ld16(t_o + c * 16, ov);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ov[i] = odd[i >> 2] >> (8 * (i & 3) + 7) & 1u ? 0x7fffffffu : ov[i];
+        tmem_st16(t_o + c * 16, ov);
+    }
+    tmem_wait_st();
+}
+
 template <class P>
 __global__ void __launch_bounds__(kThreads, 1)
 paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ P p) {
@@ -295,6 +335,7 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             }
             mbar_init(&sh->o_empty[x], kTileQ / 32);
         }
+        sh->odd_values[0] = sh->odd_values[1] = 0u;
         sh->abort_flag = 0;
         sh->tmem_base = 0xFFFFFFFFu;
         fence_mbar_init();
@@ -550,6 +591,8 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
             tc_fence_after();
             ++used;
             const float in_units = fast_exp2(unit);
+            // (Written in front of v_full, which the last P.V has waited for; item k + 2 is not there before the end of this one.)
+            if (!dead && sh->odd_values[k & 1] == k + 1) add_nan(p, p.in, sh->items[k % kItemRing], x, tok, t_o);
             if constexpr (!std::is_same<P, Whole>::value) {
                 if (it.kv0 >= 0) {  // a run of a split item: its O, maximum and sum as they are
                     float* part = p.partials + ((size_t)it.part * 2 + x) * kPartialFloats;
@@ -695,6 +738,11 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                 const int vs = t % kVSlots;
                 if (!(ok = wait_or_abort(sh, &sh->v_empty[vs], ((t / kVSlots) & 1u) ^ 1u))) break;
                 uint8_t* to = smem + kV + vs * kTileBytes + (part >> 2) * kPanelBytes + (w * 32 + r4) * 128;
+                uint32_t odd = 0;
+                if (j >= plain_tiles(it)) {
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) odd |= nan_bytes(in[s].x) | nan_bytes(in[s].y) | nan_bytes(in[s].z) | nan_bytes(in[s].w);
+                }
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {
                     const uint4 lo = make_uint4(q8::e4m3x2_to_half2(in[s].x & 0xffffu), q8::e4m3x2_to_half2(in[s].x >> 16),
@@ -706,6 +754,14 @@ paged_prefill_q8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_c
                     const int r7 = (s * 4 + r4) & 7, first = 2 * (part & 3) + (part >> 2), second = first ^ 1;
                     *reinterpret_cast<uint4*>(to + s * 512 + ((first ^ r7) << 4)) = part < 4 ? lo : hi;
                     *reinterpret_cast<uint4*>(to + s * 512 + ((second ^ r7) << 4)) = part < 4 ? hi : lo;
+                }
+                if (odd & 0x80808080u) {
+                    sh->odd_values[k & 1] = k + 1;
+#pragma unroll 1
+                    for (int i = 0; i < 128; ++i) {  // what this thread has written
+                        uint16_t* const h = reinterpret_cast<uint16_t*>(to + (i >> 4) * 512 + (((2 * (part & 3) + (i >> 3 & 1)) ^ ((i >> 4) * 4 + r4 & 7)) << 4)) + (i & 7);
+                        if ((*h & 0x7fffu) == 0x7fffu) *h = 0;
+                    }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
