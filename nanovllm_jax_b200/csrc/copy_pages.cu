@@ -87,8 +87,8 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_const
             const int64_t t = max(0, min(__ldg(p.tokens + i), p.block_size));
             live = (t * cache.rows + p.block_size - 1) / p.block_size * cache.row_bytes;
         }
-        const int bytes = (int)min((int64_t)kPieceBytes, live - off);
-        if (bytes <= 0 && off > 0) continue;  // a page's first piece looks at the pair even where nothing is live
+        const int bytes = (int)max((int64_t)0, min((int64_t)kPieceBytes, live - off));  // pages may have more than 2^31
+        if (bytes == 0 && off > 0) continue;  // a page's first piece looks at the pair even where nothing is live
         const uint8_t* const from = cache.base + s * page_bytes + off;
         uint8_t* const to = cache.base + d * page_bytes + off;
         uint4 x[kUnroll];
