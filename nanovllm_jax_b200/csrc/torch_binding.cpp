@@ -259,17 +259,29 @@ struct Site {
 };
 
 // The launches of a call go to its stream one behind the other: another thread's call on the same stream, which shares the scratch
-// buffer, must not come between them.
-std::mutex& issue_mutex() {
-    static auto* m = new std::mutex();
-    return *m;
+// buffer, must not come between them.  Calls on other streams or devices do not wait: a launch blocks while its stream takes no more
+// work, which may be until the other one's has been issued (an all-reduce of two devices driven by a thread each).
+// Looked up under the GIL; an entry stays, for its thread may be inside.
+std::mutex& issue_mutex(int device, cudaStream_t stream) {
+    struct Entry {
+        int device;
+        cudaStream_t stream;
+        std::mutex mutex;
+    };
+    static auto* list = new std::vector<Entry*>();
+    for (Entry* e : *list)
+        if (e->stream == stream && e->device == device) return e->mutex;
+    auto* e = new Entry{device, stream, {}};
+    list->push_back(e);
+    return e->mutex;
 }
 template <class F>
-void call(F&& f) {
+void call(const Site& site, F&& f) {
     int rc;
+    std::mutex& mutex = issue_mutex(site.device, site.stream);
     Py_BEGIN_ALLOW_THREADS;
     {
-        const std::lock_guard<std::mutex> lock(issue_mutex());
+        const std::lock_guard<std::mutex> lock(mutex);
         rc = f();
     }
     Py_END_ALLOW_THREADS;
@@ -355,7 +367,7 @@ PyObject* store_kvcache(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                         " tokens");
         const int64_t num_slots = flat_slots(kc, vc, kvh, d);
         const Site site(key);
-        call([&] {
+        call(site, [&] {
             return api.store_kvcache(ptr(key), ptr(value), mptr(kc), mptr(vc), iptr(slots), t, (int)kvh, (int)d, num_slots, src,
                                      site.stream);
         });
@@ -380,7 +392,7 @@ PyObject* paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor ws = a[8] == Py_None
                                   ? site.scratch(api.decode_workspace_bytes(b, h, c.kvh, c.d, mb, c.block))
                                   : tensor(a[8], "scratch");
-        call([&] {
+        call(site, [&] {
             return api.paged_decode(ptr(q), ptr(kc), ptr(vc), iptr(bt), iptr(cl), mptr(out), mptr(ws), ws.nbytes(), b, h, c.kvh,
                                     c.d, c.nb, c.block, mb, scale, site.stream);
         });
@@ -419,7 +431,7 @@ PyObject* decode_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Site site(q);
         const at::Tensor out = output_like(a[10], q);
         const at::Tensor ws = site.scratch(api.decode_workspace_bytes(b, h, c.kvh, c.d, mb, c.block));
-        call([&] {
+        call(site, [&] {
             return api.decode_step(ptr(q), ptr(key), ptr(value), mptr(kc), mptr(vc), iptr(slots), iptr(bt), iptr(cl), mptr(out),
                                    mptr(ws), ws.nbytes(), b, h, c.kvh, c.d, c.nb, c.block, mb, scale, src, site.stream);
         });
@@ -485,7 +497,7 @@ PyObject* varlen_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor out = a[6] == Py_None ? at::empty_like(q) : tensor(a[6], "out");
         zero_uncovered(host, b, out, t);
         const at::Tensor ws = site.scratch(std::max<size_t>(api.prefill_workspace_bytes(t, b, (int)h, kvh, (int)d), 256));
-        call([&] {
+        call(site, [&] {
             return api.varlen_prefill(ptr(q), ptr(k), ptr(v), iptr(cu), iptr(cu_k), host.data, mptr(out), mptr(ws), ws.nbytes(), t,
                                       b, max_seqlen, (int)h, kvh, (int)d, scale, site.stream);
         });
@@ -514,7 +526,7 @@ PyObject* paged_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor out = a[9] == Py_None ? at::empty_like(q) : tensor(a[9], "out");
         zero_uncovered(host, b, out, t);
         const at::Tensor ws = site.scratch(std::max<size_t>(api.prefill_workspace_bytes(t, b, h, c.kvh, c.d), 256));
-        call([&] {
+        call(site, [&] {
             return api.paged_prefill(ptr(q), ptr(kc), ptr(vc), iptr(cu), iptr(cu_k), iptr(bt), host.data, mptr(out), mptr(ws),
                                      ws.nbytes(), t, b, max_seqlen_q, h, c.kvh, c.d, c.nb, c.block, (int)bt.size(1), scale,
                                      site.stream);
@@ -573,7 +585,7 @@ PyObject* prefill_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor out = at::empty_like(q);
         zero_uncovered(host, b, out, t);
         const at::Tensor ws = site.scratch(std::max<size_t>(api.prefill_workspace_bytes(t, b, h, c.kvh, c.d), 256));
-        call([&] {
+        call(site, [&] {
             return api.prefill_step(ptr(q), ptr(key), ptr(value), mptr(kc), mptr(vc), iptr(slots), iptr(cu), iptr(cu_k), tables,
                                     host.data, mptr(out), mptr(ws), ws.nbytes(), t, b, max_seqlen, h, c.kvh, c.d, c.nb, c.block,
                                     mb, scale, site.stream);
@@ -612,7 +624,7 @@ PyObject* qk_norm_rope_store(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int64_t num_slots = flat_slots(kc, vc, p.kvh, p.d);
         const float eps = to_float(a[10]);
         const Site site(p.q);
-        call([&] {
+        call(site, [&] {
             return api.qk_norm_rope_store(mptr(p.q), mptr(p.key), ptr(p.value), fptr(p.q_weight), fptr(p.k_weight),
                                           fptr(p.cos_sin), iptr(p.positions), mptr(kc), mptr(vc), iptr(p.slots), p.t, (int)p.h,
                                           (int)p.kvh, (int)p.d, num_slots, p.cos_sin.size(0), eps, site.stream);
@@ -641,7 +653,7 @@ PyObject* fused_decode_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Site site(p.q);
         const at::Tensor out = a[15] == Py_None ? at::empty_like(p.q) : tensor(a[15], "out");
         const at::Tensor ws = site.scratch(api.decode_workspace_bytes(b, h, kvh, d, mb, block_size));
-        call([&] {
+        call(site, [&] {
             return api.fused_decode_step(mptr(p.q), mptr(p.key), ptr(p.value), fptr(p.q_weight), fptr(p.k_weight),
                                          fptr(p.cos_sin), iptr(p.positions), p.cos_sin.size(0), eps, mptr(kc), mptr(vc),
                                          iptr(p.slots), iptr(bt), iptr(cl), mptr(out), mptr(ws), ws.nbytes(), b, h, kvh, d,
@@ -702,7 +714,7 @@ PyObject* store_kvcache_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                         " tokens");
         const Site site(key);
         const at::Tensor ws = site.scratch(api.store_q8_workspace_bytes(t));
-        call([&] {
+        call(site, [&] {
             return api.store_kvcache_q8(ptr(key), ptr(value), mptr(c.k), mptr(c.v), (float*)mptr(c.k_scale), (float*)mptr(c.v_scale),
                                         iptr(slots), mptr(ws), ws.nbytes(), t, c.kvh, c.d, c.slots, src, site.stream);
         });
@@ -726,7 +738,7 @@ PyObject* paged_decode_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor out = output_like(a[9], q);
         same_device(q, {&out});
         const at::Tensor ws = site.scratch(api.decode_q8_workspace_bytes(b, h, c.kvh));
-        call([&] {
+        call(site, [&] {
             return api.paged_decode_q8(ptr(q), ptr(c.k), ptr(c.v), fptr(c.k_scale), fptr(c.v_scale), iptr(bt), iptr(cl), mptr(out),
                                        mptr(ws), ws.nbytes(), b, h, c.kvh, c.d, c.nb, c.block, mb, scale, site.stream);
         });
@@ -766,7 +778,7 @@ PyObject* decode_step_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor out = output_like(a[12], q);
         same_device(q, {&out});
         const at::Tensor ws = site.scratch(api.decode_q8_workspace_bytes(b, h, c.kvh));
-        call([&] {
+        call(site, [&] {
             return api.decode_step_q8(ptr(q), ptr(key), ptr(value), mptr(c.k), mptr(c.v), (float*)mptr(c.k_scale),
                                       (float*)mptr(c.v_scale), iptr(slots), iptr(bt), iptr(cl), mptr(out), mptr(ws), ws.nbytes(), b, h,
                                       c.kvh, c.d, c.nb, c.block, mb, scale, src, site.stream);
@@ -797,7 +809,7 @@ PyObject* paged_prefill_q8(PyObject*, PyObject* const* a, Py_ssize_t n) {
         same_device(q, {&out});
         zero_uncovered(host, b, out, t);
         const at::Tensor ws = site.scratch(std::max<size_t>(api.prefill_q8_workspace_bytes(t, b, h, c.kvh, c.d), 256));
-        call([&] {
+        call(site, [&] {
             return api.paged_prefill_q8(ptr(q), ptr(c.k), ptr(c.v), fptr(c.k_scale), fptr(c.v_scale), iptr(cu), iptr(cu_k), iptr(bt),
                                         host.data, mptr(out), mptr(ws), ws.nbytes(), t, b, max_seqlen_q, h, c.kvh, c.d, c.nb, c.block,
                                         (int)bt.size(1), scale, site.stream);
@@ -841,7 +853,7 @@ PyObject* copy_pages(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
             base[i] = mptr(t), rows[i] = (int32_t)t.size(1), row_bytes[i] = row;
         }
         const Site site(src);
-        call([&] {
+        call(site, [&] {
             return api.copy_pages(base.data(), rows.data(), row_bytes.data(), (int)count, iptr(src), iptr(dst),
                                   tokens ? iptr(*tokens) : nullptr, (int)src.size(0), nb, block,
                                   tables ? (int32_t*)mptr(*tables) : nullptr, tables ? tables->numel() : 0, site.stream);
