@@ -197,10 +197,25 @@ at::Tensor new_buffer(int device, size_t nbytes) {
     return at::empty({(int64_t)std::max(nbytes, (size_t)1 << 20)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
 }
 
+// Allocating may call into the runtime (memory that has to come from the driver, a question whether other streams are done with memory
+// that was given back), which ends a capture that was not begun through torch, whose allocator knows of its own captures only: nothing
+// that this thread calls meanwhile is part of the capture, so it may.
+at::Tensor new_buffer_in_capture(int device, size_t nbytes) {
+    struct Relaxed {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        Relaxed() { swap(); }
+        ~Relaxed() { swap(); }
+        void swap() {
+            if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) (void)cudaGetLastError();
+        }
+    } relaxed;
+    return new_buffer(device, nbytes);
+}
+
 const at::Tensor& captured_workspace(unsigned long long id, cudaGraph_t graph, int device, cudaStream_t stream, size_t nbytes) {
     for (Captured* c : captured())
         if (c->id == id && c->stream == stream && c->device == device && (size_t)c->buf.numel() >= nbytes) return c->buf;
-    auto* c = new Captured{id, device, stream, new_buffer(device, nbytes)};
+    auto* c = new Captured{id, device, stream, new_buffer_in_capture(device, nbytes)};
     captured().push_back(c);
     cudaUserObject_t object;
     if (cudaUserObjectCreate(&object, c, give_back, 1, cudaUserObjectNoDestructorSync) != cudaSuccess) {
