@@ -399,10 +399,10 @@ int nvllm_b200_decode_step_q8(const void* q, const void* k, const void* v, void*
  *                 nvllm_b200_varlen_prefill_workspace_bytes will do, but some calls take longer with it)
  *
  * Math: scores in fp32 from the cache's own values and from q as the sum of two e4m3 numbers under a power of two per row (exact
- * for components above 2^-11 of the row's largest, to within 2^-18 of it for smaller ones); fp16 probabilities, which carry the V
- * scale, times the cache's own values in fp16 (exact) into fp32.  What a probability loses by underflow is relative to the row's
- * largest one and to the largest V scale among the keys before it: at most 2^-32 of their product times 448; a V scale below 2^-64 of that
- * one counts as 2^-64 of it.
+ * for components from 2^-9.8 of the row's largest on, to within 2^-17.8 of it for smaller ones, where the largest is 2^-118 or more); fp16
+ * probabilities, which carry the V scale, times the cache's own values in fp16 (exact) into fp32.  What a probability loses by underflow is
+ * relative to the row's largest one and to the largest V scale among the keys before it: at most 2^-32 of their product times 448; a V scale
+ * below 2^-64 of that one counts as 2^-64 of it.
  * A NaN in the cache (what a NaN or an infinity was stored as) reaches the rows that see its token, of K every dim, of V its own.
  */
 size_t nvllm_b200_paged_prefill_q8_workspace_bytes(int64_t T, int B, int H, int KVH, int D);

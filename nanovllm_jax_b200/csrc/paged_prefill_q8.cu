@@ -7,8 +7,9 @@
 //
 //  * Q.K^T takes K as it is, e4m3 from TMA (tcgen05.mma kind::f8f6f4, K = 32 per instruction), and Q as the sum of two e4m3 tiles.
 //    bf16 has eight significant bits, e4m3 four: with a row divided by the power of two that brings its largest magnitude to
-//    224 .. 448, hi = e4m3(q) and lo = e4m3(q - hi) give every q above 2^-11 of that exactly, and a smaller one to within 2^-18 of
-//    it.  Twice as many products at twice the rate: the time of the bf16 product, with no conversion of K at all.
+//    224 .. 448, hi = e4m3(q) and lo = e4m3(q - hi) give every q from 1/4 on exactly (2^-9.8 of the largest or less) and a smaller
+//    one to within half of e4m3's least step, 2^-10 (2^-17.8 of the largest).  Twice as many products at twice the rate: the time of
+//    the bf16 product, with no conversion of K at all.
 //  * The row's power of two and the K scale of each half of a tile (a scale has 64 slots) go into the factor that the softmax
 //    multiplies its scores by anyway.
 //  * O += P.V runs in fp16 (P would lose its small probabilities in e4m3): e4m3 -> fp16 is exact and one instruction for two

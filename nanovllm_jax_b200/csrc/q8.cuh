@@ -58,7 +58,8 @@ struct RowPower {
     }
 };
 // Four elements (two words of bf16) -> upper and lower parts, a byte each: hi = e4m3(x), lo = e4m3(x - hi).  bf16 has eight
-// significant bits and e4m3 four, so the sum is exact where lo is no subnormal.
+// significant bits and e4m3 four, so the sum is exact from 1/4 on, where what hi leaves is a multiple of e4m3's least step, 2^-9; below it
+// is off by half of that step at most.
 __device__ __forceinline__ void split_row(uint32_t w0, uint32_t w1, float down, uint32_t& hi, uint32_t& lo) {
     const float f[4] = {__uint_as_float(w0 << 16) * down, __uint_as_float(w0 & 0xffff0000u) * down, __uint_as_float(w1 << 16) * down,
                   __uint_as_float(w1 & 0xffff0000u) * down};
