@@ -6,8 +6,10 @@
 //
 // Pure data movement: 2 bytes of traffic per byte copied.  A page of a tensor is cut into pieces of kPieceBytes; a CTA takes
 // one piece of one tensor (blockIdx.y: its entry of the parameters is then read by all threads at once; found by a search
-// among the pieces of all tensors, four pages of 144 tensors took 30 us instead of 13), or a few where there are many.  A CTA
-// looks through the pairs for one that forbids its own while its loads are in flight.
+// among the pieces of all tensors, four pages of 144 tensors took 30 us instead of 13).  A CTA looks through the pairs for one
+// that forbids its own while its loads are in flight: at 4096 pairs it reads as much of them as it copies, from the L2 (K and V
+// in 8 bits with their scales, 8 kv heads, pages of 256 tokens: 710 us, 0.94 of a plain copy's rate; of 64 tokens, where a page
+// is half a piece, 218 us, 0.77).  Several pieces a CTA, each with its own look, are the same within 3 %.
 #include "common.cuh"
 
 #include <algorithm>
@@ -31,8 +33,7 @@ struct Common {
     int n, block_size;
     int64_t NB;
     int pieces;        // of the largest page
-    int copy_ctas;     // per tensor; CTAs behind them take the tables
-    int64_t units;     // n * pieces
+    int copy_ctas;     // per tensor, n * pieces; CTAs behind them take the tables
     int32_t* tables;
     int64_t table_entries;
 };
@@ -56,7 +57,10 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_const
     const int tid = threadIdx.x;
     griddep_wait();
     griddep_launch_dependents();
-    if ((int)blockIdx.x >= p.copy_ctas) {  // the tables: an entry that names a source names its destination now
+    // The tables: an entry that names a source names its destination now.  A thread goes through the list for its entry, and once more for
+    // the pair that names it, the threads of a warp one after the other: 64 x 32 entries that all name one of 96 pairs 270 us, of
+    // 4096 pairs 12 ms; entries that name none cost nothing beside the copy.
+    if ((int)blockIdx.x >= p.copy_ctas) {
         const int64_t at = (int64_t)(blockIdx.x - p.copy_ctas) * kThreads + tid;
         if (blockIdx.y > 0 || at >= p.table_entries) return;
         const int page = p.tables[at];
@@ -76,45 +80,43 @@ __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_const
     const Cache cache = p.caches[blockIdx.y];
     const int64_t page_bytes = (int64_t)cache.rows * cache.row_bytes;
     const bool wide = (((uintptr_t)cache.base | (uintptr_t)cache.row_bytes) & 15) == 0;
-    for (int64_t u = blockIdx.x; u < p.units; u += p.copy_ctas) {
-        const int i = (int)(u / p.pieces);
-        const int64_t off = (u - (int64_t)i * p.pieces) * kPieceBytes;
-        if (off >= page_bytes) continue;
-        const int s = __ldg(p.src + i), d = __ldg(p.dst + i);
-        if (!in_pool(p, s) || !in_pool(p, d) || s == d) continue;
-        int64_t live = page_bytes;
-        if (p.tokens != nullptr) {
-            const int64_t t = max(0, min(__ldg(p.tokens + i), p.block_size));
-            live = (t * cache.rows + p.block_size - 1) / p.block_size * cache.row_bytes;
-        }
-        const int bytes = (int)max((int64_t)0, min((int64_t)kPieceBytes, live - off));  // pages may have more than 2^31
-        if (bytes == 0 && off > 0) continue;  // a page's first piece looks at the pair even where nothing is live
-        const uint8_t* const from = cache.base + s * page_bytes + off;
-        uint8_t* const to = cache.base + d * page_bytes + off;
-        uint4 x[kUnroll];
-        if (wide) {
+    const int i = (int)blockIdx.x / p.pieces;
+    const int64_t off = (int64_t)((int)blockIdx.x - i * p.pieces) * kPieceBytes;
+    if (off >= page_bytes) return;
+    const int s = __ldg(p.src + i), d = __ldg(p.dst + i);
+    if (!in_pool(p, s) || !in_pool(p, d) || s == d) return;
+    int64_t live = page_bytes;
+    if (p.tokens != nullptr) {
+        const int64_t t = max(0, min(__ldg(p.tokens + i), p.block_size));
+        live = (t * cache.rows + p.block_size - 1) / p.block_size * cache.row_bytes;
+    }
+    const int bytes = (int)max((int64_t)0, min((int64_t)kPieceBytes, live - off));  // pages may have more than 2^31
+    if (bytes == 0 && off > 0) return;  // a page's first piece looks at the pair even where nothing is live
+    const uint8_t* const from = cache.base + s * page_bytes + off;
+    uint8_t* const to = cache.base + d * page_bytes + off;
+    uint4 x[kUnroll];
+    if (wide) {
 #pragma unroll
-            for (int k = 0; k < kUnroll; ++k) {
-                const int at = (k * kThreads + tid) * 16;
-                if (at < bytes) x[k] = __ldg(reinterpret_cast<const uint4*>(from + at));
-            }
+        for (int k = 0; k < kUnroll; ++k) {
+            const int at = (k * kThreads + tid) * 16;
+            if (at < bytes) x[k] = __ldg(reinterpret_cast<const uint4*>(from + at));
         }
-        bool bad = false;
-        for (int j = tid; j < p.n; j += kThreads) bad |= forbids(p, j, i, d);
-        if (__syncthreads_or(bad)) {
-            if (tid == 0) atomicOr(&g_error_flag, 128);
-            continue;
-        }
-        if (wide) {
+    }
+    bool bad = false;
+    for (int j = tid; j < p.n; j += kThreads) bad |= forbids(p, j, i, d);
+    if (__syncthreads_or(bad)) {
+        if (tid == 0) atomicOr(&g_error_flag, 128);
+        return;
+    }
+    if (wide) {
 #pragma unroll
-            for (int k = 0; k < kUnroll; ++k) {
-                const int at = (k * kThreads + tid) * 16;
-                if (at < bytes) *reinterpret_cast<uint4*>(to + at) = x[k];
-            }
-        } else {  // scales of few heads: rows of 4 or 8 bytes
-            for (int at = tid * 4; at < bytes; at += kThreads * 4)
-                *reinterpret_cast<uint32_t*>(to + at) = __ldg(reinterpret_cast<const uint32_t*>(from + at));
+        for (int k = 0; k < kUnroll; ++k) {
+            const int at = (k * kThreads + tid) * 16;
+            if (at < bytes) *reinterpret_cast<uint4*>(to + at) = x[k];
         }
+    } else {  // scales of few heads: rows of 4 or 8 bytes
+        for (int at = tid * 4; at < bytes; at += kThreads * 4)
+            *reinterpret_cast<uint32_t*>(to + at) = __ldg(reinterpret_cast<const uint32_t*>(from + at));
     }
 }
 
@@ -180,11 +182,7 @@ extern "C" int nvllm_b200_copy_pages(void* const* caches_host, const int32_t* pa
         p.n = n;
         p.block_size = block_size;
         p.NB = NB;
-        p.units = count > 0 ? (int64_t)n * pieces : 0;
-        // A piece per CTA; with very many, up to 16 of them, so that the look through a long list of pairs is shared.
-        const int64_t wave = (int64_t)sm_count() * 64;
-        const int64_t each = std::max<int64_t>(1, std::min<int64_t>(16, p.units * count / wave));
-        const int64_t copy_ctas = (p.units + each - 1) / each;
+        const int64_t copy_ctas = count > 0 ? (int64_t)n * pieces : 0;
         const bool last = c0 + kMany >= num_caches;
         p.tables = last ? block_tables : nullptr;
         p.table_entries = last ? table_entries : 0;
