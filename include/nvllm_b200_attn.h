@@ -424,7 +424,7 @@ int nvllm_b200_paged_prefill_q8(const void* q, const void* k_cache, const void* 
  *   tokens        [n] int32 or NULL: only the rows of the first tokens[i] tokens are copied (0 .. block_size); the other
  *                 rows of the destination stay as they are
  *   block_tables  int32, table_entries of them, or NULL: every entry that names a source is set to its destination (the
- *                 first such pair's)
+ *                 first such pair's that is carried out)
  *
  * Pairs are independent: the pages read hold what they held before the call.  A pair whose destination another pair reads
  * from, or a later pair writes to, is left out (its table entries stay, too), and bit 7 (128) of the device status is raised.

@@ -25,11 +25,12 @@
 // 128 x 64 x 32 byte product reads 6 KB of shared memory, 48 cycles for 32 of arithmetic.  Left out one by one (wrong results, to see
 // what counts): the lower part of Q 575 us, three quarters of P.V 555, both and the rest of Q.K^T 520; the exponentials 641 and
 // without all of the products 408; the conversion 636; the V loads 627.
-// Measured instead: V bytes staged by TMA and written as bf16 668 (12 sequences of 17..700 tokens behind 500..5000: 303, now 254);
-// steps of 128 keys and one score buffer 638 (276); the next step's scores taken into registers before this one's exponentials 767
-// (324); sixteen softmax warps, two threads a row 707 (291); a share of the exponentials as polynomials 686 (an eighth) .. 744 (a quarter);
-// probabilities against the maximum of the steps before while this one's is found, taken again where it grew 657 (267); V converted by
-// integer operations instead of cvt 654.
+// Measured instead, each against the form of its time: V bytes staged by TMA and written as bf16 668 (12 sequences of 17..700 tokens
+// behind 500..5000: 303; as it is now 240 to 283, by box and clock); steps of 128 keys and one score buffer 638 (276) when steps of 64
+// took 649 (262), with a commit per P.V and K slots given back by the issuers; the next step's scores taken into registers before this
+// one's exponentials 767 (324); sixteen softmax warps, two threads a row 707 (291); a share of the exponentials as polynomials 686 (an
+// eighth) .. 744 (a quarter); probabilities against the maximum of the steps before while this one's is found, taken again where it grew
+// 657 (267); V converted by integer operations instead of cvt 654.
 //
 // Per CTA (16 warps = 4 warpgroups; registers 96 | 160 | 160 | 96 of the launch's 128 each):
 //   warp 0       TMA producer: K bytes, four slots; slot and scales of a tile, looked up a tile ahead, into a ring

@@ -323,8 +323,8 @@ __device__ __forceinline__ Item load_item(const SplitParams& p, const List& l, i
 
 // A few rounds of items, each an SM's work for a long time: those of the last round, which leaves SMs idle, are cut into runs as well.  `ctas`:
 // the launch's, which claim the items in their order and then the runs.  (8-bit pages only: packed bf16 keys and bf16 keys in pages
-// are to give the same bits.)  Whole and cut, 32 / 8 heads: 1280 new tokens (160 items) behind 30 000 1058 and 665 us, behind 8000 310 and 216,
-// behind 2500 130 and 120; 640 (80 items) behind 8000 158 and 142; 2560 (320) 479 and 432; 20 x 64 behind 3000 127 and 110.  Twice the room
+// are to give the same bits.)  Whole and cut, 32 / 8 heads: 1280 new tokens (160 items) behind 30 000 1044 and 637 us, behind 8000 304 and 225,
+// behind 2500 121 and 117; 640 (80 items) behind 8000 157 and 143; 2560 (320) 473 and 410; 20 x 64 behind 3000 126 and 113.  Twice the room
 // for results lets 2048 (256) be cut, too: 345 instead of 335, for at the power cap what idle SMs leave makes the others faster.
 struct TailParams : Params {
     float* partials;  // [kTailSlots * ctas][Q tile][kPartialFloats]
