@@ -104,3 +104,17 @@ def test_stored_infinities_do_not_reach_earlier_tokens():
         out = ops.paged_prefill_q8(q, *cache, tables, cu, cu_k, 50, 0.0884, 128)
         assert out[:49].isfinite().all()
     assert out[49, :4, 7].isnan().all() and out[49, 4:, 9].isnan().all() and int(out.isnan().sum()) == 8
+
+
+@pytest.mark.parametrize("h, kvh, new, pre", [(32, 8, 2048, 700), (3, 1, 700, 5000), (8, 1, 40, 9000)])
+def test_values_of_nothing_but_nan(h, kvh, new, pre):
+    """Every row has to look for its own in every tile that it shares: no wait runs out meanwhile."""
+    import torch
+    from nanovllm_jax_b200 import _lib, ops
+    rng = np.random.default_rng(h)
+    q, tables, cu, cu_k, _, nb, _ = make(rng, [new], [pre], h, kvh, 128)
+    cache = random_cache(rng, nb, 128, kvh)
+    cache[1].view(torch.uint8)[:, :, 0] = 0x7f
+    out = ops.paged_prefill_q8(q, *cache, tables, cu, cu_k, new, 0.0884, 128)
+    assert out[:, :h // kvh].isnan().all() and out[:, h // kvh:].isfinite().all()
+    assert _lib.device_status() == 0
